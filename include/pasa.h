@@ -50,7 +50,7 @@
 extern "C" {
 #endif
 
-#define PASA_ABI_VERSION 12
+#define PASA_ABI_VERSION 13
 
 typedef enum {
   PASA_OK = 0,
@@ -417,6 +417,108 @@ int pasa_row_ops(const void* x, int x_dtype,
                  void* y, int y_dtype,
                  int64_t rows, int64_t cols, int64_t rows_per_batch, int64_t param_stride,
                  double eps, void* stream);
+
+/* ---- Rotary embedding from positions on several axes -------------------------- */
+
+typedef enum { PASA_POS_I32 = 0, PASA_POS_I64 = 1, PASA_POS_F32 = 2 } pasa_pos_type_t;
+
+typedef enum {
+  PASA_PAIRS_INTERLEAVED = 0, /* pair i is channels (2 i, 2 i + 1)     */
+  PASA_PAIRS_HALVES = 1       /* pair i is channels (i, i + pairs)     */
+} pasa_pairing_t;
+
+/* q or k and where its rotation goes: element (b, s, h, d) lies at stride[0] b + stride[1] s + stride[2] h + d. */
+typedef struct {
+  const void* in;
+  void* out;             /* may be `in` with equal strides (in place); no other overlap */
+  int64_t in_stride[3];
+  int64_t out_stride[3];
+  int64_t heads;
+} pasa_rope_tensor_t;
+
+/* Pair i of every head of token (b, s) turns by a = positions[axis_of_pair[i]][b][s] * inv_freq[i] radians:
+ *   y0 = x0 cos a - x1 sin a,  y1 = x1 cos a + x0 sin a;   with `inverse` by -a, which is the gradient.
+ * Channels from 2 * pairs on are copied.  The angle is reduced in fp64, the rotation is fp32 and rounded once to
+ * `dtype` (bf16, fp16 or fp32).  positions: int32, int64 or fp32, element (axis, b, s) at pos_axis_stride axis +
+ * pos_batch_stride b + pos_seq_stride s.  inv_freq: fp64 [pairs]; axis_of_pair: int32 [pairs], each in [0, axes) (one
+ * outside is taken as the nearest).  k may be NULL.  head_dim 2 .. 256.  Any strides and alignment; rows whose
+ * 16-byte chunks are aligned move 16 bytes at a time. */
+int pasa_rope_axes(const pasa_rope_tensor_t* q, const pasa_rope_tensor_t* k, const void* positions, int pos_type,
+                   int64_t pos_axis_stride, int64_t pos_batch_stride, int64_t pos_seq_stride, int64_t axes,
+                   const double* inv_freq, const int32_t* axis_of_pair, int64_t pairs, int64_t batch, int64_t seq_len,
+                   int64_t head_dim, int pairing, int inverse, int dtype, void* stream);
+
+/* ---- Key/value cache in 8 bits ------------------------------------------------ */
+
+/* num_pages pages of page_size tokens (a power of two, 16 .. 128) for each of `heads` key heads:
+ *   k [num_pages][heads][page_size][dim], v [num_pages][heads][dim][page_size]: e4m3 codes (16-byte aligned)
+ *   k_exp, v_exp [num_pages][heads]: int8; a value is its code times 2 ** exponent, -50 <= exponent <= 50
+ * dim: 64 or 128.  Channels from head_dim on hold zero codes. */
+typedef struct {
+  void* k;
+  void* v;
+  void* k_exp;
+  void* v_exp;
+  int64_t num_pages, heads, page_size, dim, head_dim;
+} pasa_kv8_t;
+
+/* Block tables, slots and positions of a step, on the GPU, from the requests' lengths.
+ * Request r has lens[r] cached tokens and new_tokens[r] new ones (negative: 0); its pages are block_tables[r][0 ..
+ * ceil(lens[r] / page_size)).  It takes ceil((lens + new) / page_size) - ceil(lens / page_size) more from the end of
+ * free_pages[0 .. num_free[0]), requests in order, and writes them behind the ones it has.
+ *   cu_q [requests + 1]  first new token of each request: min(tokens, the sum before it)
+ *   slots [tokens]       page * page_size + offset of each new token, -1 where it has no page
+ *   positions [tokens]   lens[r] + its number in its request
+ *   lens_out [requests]  tokens that have a page: lens + new, but where the free list or the table's width ends
+ *   num_free_out [1]     pages left at the front of free_pages
+ * Tokens from cu_q[requests] on get slot and position -1.  free_pages, lens and num_free are not written; lens_out and
+ * num_free_out are other buffers.  At most 4096 requests. */
+int pasa_block_tables(int32_t* block_tables, int64_t table_stride, int64_t width, const int32_t* lens,
+                      const int32_t* new_tokens, int64_t requests, const int32_t* free_pages, int64_t free_capacity,
+                      const int32_t* num_free, int64_t page_size, int64_t tokens, int32_t* cu_q, int64_t* slots,
+                      int32_t* positions, int32_t* lens_out, int32_t* num_free_out, void* stream);
+
+/* k and v [tokens, heads, head_dim] (bf16, fp16 or fp32; strides in elements, channels contiguous) into the cache at
+ * slots[t] (negative or past the cache: skipped).  Tokens in a row whose slots follow each other inside one page are a
+ * run.  A page's exponent is the smallest e with amax <= 448 * 2 ** e over the finite values of the run, clamped to
+ * [-50, 50]; a run that does not begin at the page's first slot keeps at least the page's exponent, and where that
+ * rises the page's other codes are scaled to it.  A run at the first slot begins the page anew.  Codes are rounded to
+ * nearest even; magnitudes above 448 * 2 ** 50 become that, what is not finite is stored as NaN.  One call writes a page
+ * in one run: the contents of a page that two runs of one call write are unspecified. */
+int pasa_kv8_append(const pasa_kv8_t* cache, const void* k, const void* v, const int64_t* slots, int64_t tokens,
+                    int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                    int dtype, void* stream);
+
+/* One call of pasa_kv8_attn. */
+typedef struct {
+  const void* q;                 /* [tokens, q_heads, head_dim] bf16 or fp16, channels contiguous   */
+  void* o;                       /* likewise                                                         */
+  float* lse;                    /* [tokens, q_heads]: log of the row's sum (natural), or NULL      */
+  int64_t q_token_stride, q_head_stride, o_token_stride, o_head_stride; /* elements                  */
+  const int32_t* block_tables;   /* [requests, width], rows table_stride apart; -1: no page         */
+  int64_t table_stride, width;
+  const int32_t* lens;           /* [requests]: cached tokens, the new ones included                 */
+  const int32_t* cu_q;           /* [requests + 1]: first row of each request; NULL: tokens / requests each */
+  int64_t tokens, requests, q_heads;
+  int64_t max_kv;                /* keys from here on are not looked at                             */
+  int64_t window;                /* 0: none                                                         */
+  int causal;
+  int zero_tail;                 /* rows behind the last request become 0 (lse: -inf); else left as they were */
+  int dtype;
+  double scale;                  /* of the scores, in [1e-20, 1e20]                                 */
+} pasa_kv8_attn_t;
+
+/* Bytes of workspace (16-byte aligned) that pasa_kv8_attn needs for these sizes; 0 if none. */
+size_t pasa_kv8_attn_workspace_bytes(int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                     int64_t max_kv);
+
+/* Softmax attention of the requests' new tokens to the cache.  Row i of request r, at position lens[r] - n_r + i, sees
+ * the keys j < lens[r] with j <= position if causal, j > position - window if window > 0, and a page: a table entry
+ * outside [0, num_pages) hides its page's keys.  A row that sees nothing is 0.  q_heads is a multiple of the cache's
+ * heads; query head h reads key head h / (q_heads / heads).  What lies in the cache behind a request's last key, or
+ * under keys that a row does not see, does not reach the row, NaN included.  Softmax statistics and sums are fp32. */
+int pasa_kv8_attn(const pasa_kv8_t* cache, const pasa_kv8_attn_t* args, void* workspace, size_t workspace_bytes,
+                  void* stream);
 
 #ifdef __cplusplus
 }

@@ -46,7 +46,33 @@ class Placement(ctypes.Structure):
                 ("head_is_temporal", ctypes.c_void_p), ("heads", ctypes.c_int64)]
 
 
+class RopeTensor(ctypes.Structure):
+    """pasa_rope_tensor_t: a tensor to rotate and where its rotation goes."""
+    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("in_stride", ctypes.c_int64 * 3),
+                ("out_stride", ctypes.c_int64 * 3), ("heads", ctypes.c_int64)]
+
+
+class Kv8(ctypes.Structure):
+    """pasa_kv8_t: a key/value cache in 8 bits."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_exp", "v_exp")] + \
+               [(n, ctypes.c_int64) for n in ("num_pages", "heads", "page_size", "dim", "head_dim")]
+
+
+class Kv8Attn(ctypes.Structure):
+    """pasa_kv8_attn_t: one call of pasa_kv8_attn."""
+    _fields_ = [("q", ctypes.c_void_p), ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+                ("o_token_stride", ctypes.c_int64), ("o_head_stride", ctypes.c_int64),
+                ("block_tables", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("width", ctypes.c_int64),
+                ("lens", ctypes.c_void_p), ("cu_q", ctypes.c_void_p),
+                ("tokens", ctypes.c_int64), ("requests", ctypes.c_int64), ("q_heads", ctypes.c_int64),
+                ("max_kv", ctypes.c_int64), ("window", ctypes.c_int64), ("causal", ctypes.c_int),
+                ("zero_tail", ctypes.c_int), ("dtype", ctypes.c_int), ("scale", ctypes.c_double)]
+
+
 _pl = ctypes.POINTER(Placement)
+_rt = ctypes.POINTER(RopeTensor)
+_kv = ctypes.POINTER(Kv8)
 
 # name -> (restype, argtypes); mirrors include/pasa.h exactly.
 SIGNATURES = {
@@ -84,9 +110,16 @@ SIGNATURES = {
                                  _i64, _i64, _int, _int, _dbl, _vp, _vp, _int, _i64, _int, _vp]),
     "pasa_row_ops": (_int, [_vp, _int, _vp, _int, _vp, _vp, _int, _int, _vp, _vp, _int, _vp, _vp, _vp, _int,
                             _i64, _i64, _i64, _i64, _dbl, _vp]),
+    "pasa_rope_axes": (_int, [_rt, _rt, _vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _int,
+                              _int, _int, _vp]),
+    "pasa_block_tables": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp,
+                                 _vp]),
+    "pasa_kv8_append": (_int, [_kv, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int, _vp]),
+    "pasa_kv8_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "pasa_kv8_attn": (_int, [_kv, ctypes.POINTER(Kv8Attn), _vp, _sz, _vp]),
 }
 
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 # Size of the static device array behind pasa_sparse_attn_noalloc (PASA_NOALLOC_SCRATCH_BYTES).
 NOALLOC_SCRATCH_BYTES = 64 << 20
@@ -138,3 +171,13 @@ def call(fn: str, *args) -> int:
     rc = getattr(load(), fn)(*args)
     check(fn, rc)
     return rc
+
+
+def shares_memory(t) -> bool:
+    """Whether two elements of the tensor ``t`` may share memory."""
+    reach = 1
+    for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
+        if stride < reach:
+            return True
+        reach = stride * (size - 1) + reach
+    return False

@@ -12,6 +12,7 @@
 
 #include "../../include/pasa.h"
 #include "kernels.h"
+#include "kv_cache.h"
 
 namespace {
 
@@ -878,6 +879,220 @@ int pasa_row_ops(const void* x, int x_dtype, const void* residual, int residual_
   p.ln = layernorm != 0;
   p.eps = (float)eps;
   return launch_status(pasa::launch_row_ops(p, (hipStream_t)stream), "pasa_row_ops");
+}
+
+/* ---- positions, block tables and the key/value cache in 8 bits ---------------------- */
+
+static int check_rope_tensor(const pasa_rope_tensor_t* t, const char* name) {
+  if (!t->in || !t->out) return fail(PASA_ERR_NULL_POINTER, "pasa_rope_axes: %s has a NULL pointer", name);
+  if (t->heads < 1) return fail(PASA_ERR_BAD_SHAPE, "pasa_rope_axes: %s has %lld heads", name, (long long)t->heads);
+  if (t->heads > 65535) return fail(PASA_ERR_OVERFLOW, "pasa_rope_axes: %s has %lld heads (at most 65535)", name, (long long)t->heads);
+  return PASA_OK;
+}
+
+int pasa_rope_axes(const pasa_rope_tensor_t* q, const pasa_rope_tensor_t* k, const void* positions, int pos_type,
+                   int64_t pos_axis_stride, int64_t pos_batch_stride, int64_t pos_seq_stride, int64_t axes,
+                   const double* inv_freq, const int32_t* axis_of_pair, int64_t pairs, int64_t batch, int64_t seq_len,
+                   int64_t head_dim, int pairing, int inverse, int dtype, void* stream) {
+  int rc;
+  if (!q) return fail(PASA_ERR_NULL_POINTER, "pasa_rope_axes: q is NULL");
+  if (batch < 0 || seq_len < 0) return fail(PASA_ERR_BAD_SHAPE, "pasa_rope_axes: batch=%lld, seq_len=%lld", (long long)batch, (long long)seq_len);
+  if (batch == 0 || seq_len == 0) return ok();
+  if ((rc = check_rope_tensor(q, "q"))) return rc;
+  if (k && (rc = check_rope_tensor(k, "k"))) return rc;
+  if (!positions || !inv_freq || !axis_of_pair) return fail(PASA_ERR_NULL_POINTER, "pasa_rope_axes: NULL pointer");
+  if ((rc = check_any_dtype(dtype, "pasa_rope_axes"))) return rc;
+  if (pos_type != PASA_POS_I32 && pos_type != PASA_POS_I64 && pos_type != PASA_POS_F32)
+    return fail(PASA_ERR_DTYPE, "pasa_rope_axes: positions of type %d", pos_type);
+  if (head_dim < 2 || head_dim > 256) return fail(PASA_ERR_HEAD_DIM, "pasa_rope_axes: head_dim %lld not in [2, 256]", (long long)head_dim);
+  if (pairs < 1 || 2 * pairs > head_dim)
+    return fail(PASA_ERR_BAD_SHAPE, "pasa_rope_axes: %lld pairs in head_dim %lld", (long long)pairs, (long long)head_dim);
+  if (axes < 1 || axes > 65535) return fail(PASA_ERR_BAD_SHAPE, "pasa_rope_axes: %lld axes", (long long)axes);
+  if (pairing != PASA_PAIRS_INTERLEAVED && pairing != PASA_PAIRS_HALVES)
+    return fail(PASA_ERR_BAD_ARG, "pasa_rope_axes: pairing %d", pairing);
+  if (inverse != 0 && inverse != 1) return fail(PASA_ERR_BAD_ARG, "pasa_rope_axes: inverse must be 0 or 1");
+  if (batch > kMaxI32 / seq_len) return fail(PASA_ERR_OVERFLOW, "pasa_rope_axes: batch*seq_len overflows");
+  pasa::RopeAxesParams p{};
+  const pasa_rope_tensor_t* ts[2] = {q, k};
+  for (int i = 0; i < 2; ++i) {
+    if (!ts[i]) continue;
+    p.t[i] = {ts[i]->in, ts[i]->out, ts[i]->in_stride[0], ts[i]->in_stride[1], ts[i]->in_stride[2],
+              ts[i]->out_stride[0], ts[i]->out_stride[1], ts[i]->out_stride[2], (int)ts[i]->heads};
+  }
+  p.pos = positions;
+  p.pos_type = pos_type;
+  p.pos_axis = pos_axis_stride;
+  p.pos_b = pos_batch_stride;
+  p.pos_s = pos_seq_stride;
+  p.inv_freq = inv_freq;
+  p.axis = axis_of_pair;
+  p.axes = (int)axes;
+  p.B = batch;
+  p.S = seq_len;
+  p.D = (int)head_dim;
+  p.pairs = (int)pairs;
+  p.halves = pairing == PASA_PAIRS_HALVES;
+  p.inverse = inverse;
+  p.dtype = dtype;
+  return launch_status(pasa::launch_rope_axes(p, (hipStream_t)stream), "pasa_rope_axes");
+}
+
+static int check_page_size(int64_t page_size, const char* what) {
+  if (page_size < 16 || page_size > 128 || (page_size & (page_size - 1)))
+    return fail(PASA_ERR_BLOCK_SIZE, "%s: page_size %lld is not a power of two in [16, 128]", what, (long long)page_size);
+  return PASA_OK;
+}
+
+int pasa_block_tables(int32_t* block_tables, int64_t table_stride, int64_t width, const int32_t* lens,
+                      const int32_t* new_tokens, int64_t requests, const int32_t* free_pages, int64_t free_capacity,
+                      const int32_t* num_free, int64_t page_size, int64_t tokens, int32_t* cu_q, int64_t* slots,
+                      int32_t* positions, int32_t* lens_out, int32_t* num_free_out, void* stream) {
+  int rc;
+  if (requests < 1 || width < 1 || tokens < 0 || free_capacity < 0 || table_stride < width)
+    return fail(PASA_ERR_BAD_SHAPE, "pasa_block_tables: requests=%lld, width=%lld, table_stride=%lld, tokens=%lld, free_capacity=%lld",
+                (long long)requests, (long long)width, (long long)table_stride, (long long)tokens, (long long)free_capacity);
+  if (requests > pasa::kMaxTableRequests)
+    return fail(PASA_ERR_OVERFLOW, "pasa_block_tables: %lld requests (at most %d)", (long long)requests, pasa::kMaxTableRequests);
+  if (tokens > kMaxI32 || width > kMaxI32 || free_capacity > kMaxI32)
+    return fail(PASA_ERR_OVERFLOW, "pasa_block_tables: sizes above 2^31 - 1");
+  if (!block_tables || !lens || !new_tokens || !num_free || !cu_q || !lens_out || !num_free_out || (free_capacity > 0 && !free_pages) ||
+      (tokens > 0 && (!slots || !positions)))
+    return fail(PASA_ERR_NULL_POINTER, "pasa_block_tables: NULL pointer");
+  if (lens == lens_out || num_free == num_free_out)
+    return fail(PASA_ERR_BAD_ARG, "pasa_block_tables: lens_out and num_free_out must not be the inputs");
+  if ((rc = check_page_size(page_size, "pasa_block_tables"))) return rc;
+  pasa::KvTablesParams p{};
+  p.tables = block_tables;
+  p.stride = table_stride;
+  p.width = width;
+  p.lens = lens;
+  p.new_tokens = new_tokens;
+  p.requests = (int)requests;
+  p.free_pages = free_pages;
+  p.free_cap = free_capacity;
+  p.num_free = num_free;
+  p.page_log2 = __builtin_ctzll((unsigned long long)page_size);
+  p.tokens = tokens;
+  p.cu_q = cu_q;
+  p.slots = slots;
+  p.positions = positions;
+  p.lens_out = lens_out;
+  p.num_free_out = num_free_out;
+  return launch_status(pasa::launch_kv_tables(p, (hipStream_t)stream), "pasa_block_tables");
+}
+
+static int check_cache(const pasa_kv8_t* c, const char* what, pasa::KvCache* out) {
+  int rc;
+  if (!c || !c->k || !c->v || !c->k_exp || !c->v_exp) return fail(PASA_ERR_NULL_POINTER, "%s: the cache has a NULL pointer", what);
+  if (c->dim != 64 && c->dim != 128) return fail(PASA_ERR_HEAD_DIM, "%s: the cache's dim %lld not in {64, 128}", what, (long long)c->dim);
+  if (c->head_dim < 1 || c->head_dim > c->dim)
+    return fail(PASA_ERR_HEAD_DIM, "%s: head_dim %lld not in [1, %lld]", what, (long long)c->head_dim, (long long)c->dim);
+  if ((rc = check_page_size(c->page_size, what))) return rc;
+  if (c->num_pages < 1 || c->heads < 1) return fail(PASA_ERR_BAD_SHAPE, "%s: %lld pages of %lld heads", what, (long long)c->num_pages, (long long)c->heads);
+  if (c->num_pages > kMaxI32 || c->heads > kMaxGridY)
+    return fail(PASA_ERR_OVERFLOW, "%s: %lld pages of %lld heads", what, (long long)c->num_pages, (long long)c->heads);
+  if (((uintptr_t)c->k | (uintptr_t)c->v) & 15u) return fail(PASA_ERR_BAD_ARG, "%s: the cache's k and v must be 16-byte aligned", what);
+  out->k = (uint8_t*)c->k;
+  out->v = (uint8_t*)c->v;
+  out->k_exp = (int8_t*)c->k_exp;
+  out->v_exp = (int8_t*)c->v_exp;
+  out->num_pages = (int)c->num_pages;
+  out->heads = (int)c->heads;
+  out->page_log2 = __builtin_ctzll((unsigned long long)c->page_size);
+  out->dim = (int)c->dim;
+  out->head_dim = (int)c->head_dim;
+  return PASA_OK;
+}
+
+int pasa_kv8_append(const pasa_kv8_t* cache, const void* k, const void* v, const int64_t* slots, int64_t tokens,
+                    int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                    int dtype, void* stream) {
+  int rc;
+  pasa::KvAppendParams p{};
+  if ((rc = check_cache(cache, "pasa_kv8_append", &p.c))) return rc;
+  if ((rc = check_any_dtype(dtype, "pasa_kv8_append"))) return rc;
+  if (tokens < 0) return fail(PASA_ERR_BAD_SHAPE, "pasa_kv8_append: tokens=%lld", (long long)tokens);
+  if (tokens > kMaxI32) return fail(PASA_ERR_OVERFLOW, "pasa_kv8_append: tokens=%lld too large", (long long)tokens);
+  if (tokens == 0) return ok();
+  if (!k || !v || !slots) return fail(PASA_ERR_NULL_POINTER, "pasa_kv8_append: NULL pointer");
+  p.x[0] = k;
+  p.x[1] = v;
+  p.tok_stride[0] = k_token_stride;
+  p.tok_stride[1] = v_token_stride;
+  p.head_stride[0] = k_head_stride;
+  p.head_stride[1] = v_head_stride;
+  p.slots = slots;
+  p.tokens = tokens;
+  p.dtype = dtype;
+  return launch_status(pasa::launch_kv_append(p, (hipStream_t)stream), "pasa_kv8_append");
+}
+
+static int check_kv8_attn_sizes(int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_kv) {
+  if (tokens < 0 || requests < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || max_kv < 0)
+    return fail(PASA_ERR_BAD_SHAPE, "pasa_kv8_attn: tokens=%lld, requests=%lld, q_heads=%lld (a multiple of %lld), max_kv=%lld",
+                (long long)tokens, (long long)requests, (long long)q_heads, (long long)kv_heads, (long long)max_kv);
+  if (requests > kMaxI32 / 2 || q_heads > kMaxGridY || tokens > kMaxI32 / q_heads)
+    return fail(PASA_ERR_OVERFLOW, "pasa_kv8_attn: tokens=%lld of %lld heads, requests=%lld", (long long)tokens, (long long)q_heads, (long long)requests);
+  return PASA_OK;
+}
+
+size_t pasa_kv8_attn_workspace_bytes(int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                     int64_t max_kv) {
+  if (check_kv8_attn_sizes(tokens, requests, q_heads, kv_heads, max_kv) || tokens == 0) return 0;
+  const pasa::KvAttnPlan plan = pasa::kv_attn_plan(tokens, (int)requests, (int)q_heads, (int)kv_heads, max_kv);
+  return plan.splits == 1 ? 0 : (size_t)plan.splits * (size_t)(tokens * q_heads) * (size_t)(dim + 2) * sizeof(float);
+}
+
+int pasa_kv8_attn(const pasa_kv8_t* cache, const pasa_kv8_attn_t* a, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  pasa::KvAttnParams p{};
+  if ((rc = check_cache(cache, "pasa_kv8_attn", &p.c))) return rc;
+  if (!a) return fail(PASA_ERR_NULL_POINTER, "pasa_kv8_attn: NULL pointer");
+  if ((rc = check_kv8_attn_sizes(a->tokens, a->requests, a->q_heads, cache->heads, a->max_kv))) return rc;
+  if (a->dtype != PASA_DTYPE_BF16 && a->dtype != PASA_DTYPE_F16)
+    return fail(PASA_ERR_DTYPE, "pasa_kv8_attn: dtype %d is not bf16 or fp16", a->dtype);
+  if (!(a->scale >= 1e-20 && a->scale <= 1e20)) return fail(PASA_ERR_BAD_ARG, "pasa_kv8_attn: scale must be in [1e-20, 1e20]");
+  if (a->window < 0) return fail(PASA_ERR_BAD_ARG, "pasa_kv8_attn: window=%lld", (long long)a->window);
+  if (a->width < 1 || a->table_stride < a->width)
+    return fail(PASA_ERR_BAD_SHAPE, "pasa_kv8_attn: width=%lld, table_stride=%lld", (long long)a->width, (long long)a->table_stride);
+  if (a->width > kMaxI32) return fail(PASA_ERR_OVERFLOW, "pasa_kv8_attn: width=%lld too large", (long long)a->width);
+  if (a->cu_q == nullptr && a->tokens % a->requests)
+    return fail(PASA_ERR_BAD_SHAPE, "pasa_kv8_attn: %lld tokens are not the same number for each of %lld requests", (long long)a->tokens, (long long)a->requests);
+  if (a->tokens == 0) return ok();
+  if (!a->q || !a->o || !a->block_tables || !a->lens) return fail(PASA_ERR_NULL_POINTER, "pasa_kv8_attn: NULL pointer");
+  const size_t need = pasa_kv8_attn_workspace_bytes(a->tokens, a->requests, a->q_heads, cache->heads, cache->dim, a->max_kv);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(PASA_ERR_WORKSPACE, "pasa_kv8_attn: workspace %zu bytes < %zu", workspace ? workspace_bytes : (size_t)0, need);
+  if (need > 0 && ((uintptr_t)workspace & 15u)) return fail(PASA_ERR_BAD_ARG, "pasa_kv8_attn: workspace must be 16-byte aligned");
+  const pasa::KvAttnPlan plan = pasa::kv_attn_plan(a->tokens, (int)a->requests, (int)a->q_heads, (int)cache->heads, a->max_kv);
+  p.q = a->q;
+  p.o = a->o;
+  p.lse = a->lse;
+  p.q_tok = a->q_token_stride;
+  p.q_head = a->q_head_stride;
+  p.o_tok = a->o_token_stride;
+  p.o_head = a->o_head_stride;
+  p.tables = a->block_tables;
+  p.table_stride = a->table_stride;
+  p.width = a->width;
+  p.lens = a->lens;
+  p.cu_q = a->cu_q;
+  p.requests = (int)a->requests;
+  p.tokens = a->tokens;
+  p.q_heads = (int)a->q_heads;
+  p.group = (int)(a->q_heads / cache->heads);
+  p.max_kv = a->max_kv;
+  p.window = a->window;
+  p.causal = a->causal != 0;
+  p.zero_tail = a->zero_tail != 0;
+  p.q_vec = (((uintptr_t)a->q & 15u) == 0) && ((a->q_token_stride | a->q_head_stride) & 7) == 0;
+  p.o_vec = (((uintptr_t)a->o & 7u) == 0) && ((a->o_token_stride | a->o_head_stride) & 3) == 0;
+  p.scale = (float)(a->scale * 1.4426950408889634);
+  p.f16 = a->dtype == PASA_DTYPE_F16;
+  p.splits = plan.splits;
+  p.part_o = (float*)workspace;
+  p.part_ml = p.part_o == nullptr ? nullptr : p.part_o + (size_t)plan.splits * (size_t)(a->tokens * a->q_heads) * (size_t)cache->dim;
+  return launch_status(pasa::launch_kv_attn(p, (hipStream_t)stream), "pasa_kv8_attn");
 }
 
 }  // extern "C"

@@ -1,0 +1,466 @@
+// Softmax attention to the key/value cache in 8 bits.
+//
+// Request r has n new tokens (rows of q) and len[r] cached ones, its own included.  Token i of it sits at position
+// pos = len - n + i and sees the keys j with j < len, j <= pos if causal, j > pos - window with a window, and a page in
+// the table.  With a page's exponents ke, ve:
+//   s_j = scale 2^ke q.k8_j,   o = sum_j 2^(s_j - m) 2^ve v8_j / sum_j 2^(s_j - m)        (scale holds log2 e)
+// m is the running maximum of s_j + ve, so that p_j = 2^(s_j + ve - m + 15) <= 2^15 carries the page's scale and stays
+// inside fp16's normal numbers down to 2^-29 of the largest; the row sum takes p_j 2^-ve, which is exact.
+// Rows that see no key get 0, and -inf as the logarithm of their sum.
+//
+// The codes go to the matrix unit as they lie in memory.  Both products contract over what is contiguous in the cache,
+// and a contraction may run in any order, so a lane's operand is 16 consecutive bytes, widened in registers: e4m3 is
+// exact in both 16-bit types.  q.k runs in q's type, p.v in fp16 whatever q's type is: p then has 11 bits, not 8.
+// Per 64-key tile, lane (m, g) = (lane % 16, lane / 16):
+//   S^T = K Q^T   A row m of 16-key tile t is key 16 (m / 4) + 4 t + m % 4, so that the lane's 16 results are
+//                 keys 16 g .. 16 g + 15 of row m of q: one page, one pair of exponents
+//   O^T += V^T P^T  A row m of 16-channel tile dt is channel 16 dt + m, k-slots keys 16 g + 8 u .. + 7 of step u:
+//                 the lane's own results as they stand, and 16 bytes of V
+#include <type_traits>
+
+#include "common.h"
+#include "kv_cache.h"
+
+namespace pasa {
+
+namespace {
+
+constexpr float kShift = 15.f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+// Eight e4m3 codes as eight values of a 16-bit type, exactly.
+__device__ __forceinline__ f16x8_t widen_f16(uint32_t lo, uint32_t hi) {
+  const f16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+  const f16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+  const f16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+  const f16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+  return (f16x8_t){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ bf16x8_t widen_bf16(uint32_t lo, uint32_t hi) {
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  return (bf16x8_t){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+template <typename E>
+__device__ __forceinline__ typename E::vec8 widen(uint32_t lo, uint32_t hi) {
+  if constexpr (std::is_same_v<E, F16>) return widen_f16(lo, hi);
+  else return widen_bf16(lo, hi);
+}
+
+// A byte mask of the first n (0 .. 4) bytes of a word.
+__device__ __forceinline__ uint32_t first_bytes(int n) {
+  return n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+}
+// 0x80 in each byte that is e4m3's NaN (0x7f or 0xff).
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// The requests' first rows of q, clamped to the rows that there are.
+__device__ __forceinline__ int64_t first_token(const KvAttnParams& p, int r) {
+  if (p.cu_q == nullptr) return (int64_t)r * (p.tokens / p.requests);
+  return min(max((int64_t)p.cu_q[r], (int64_t)0), p.tokens);
+}
+
+// Tile `id` of the launch: request r (requests: the rows behind the last one), and its first row.  The tiles of a
+// request are numbered from floor(first row / TILE) + r, which leaves room for every request's last, part-filled one
+// without a sum over the requests before it.
+template <int TILE>
+__device__ __forceinline__ int find_tile(const KvAttnParams& p, int64_t id, int64_t& tok0, int64_t& rows, int64_t& row0) {
+  int lo = 0, hi = p.requests + 1;
+  auto start = [&](int r) { return first_token(p, r) * p.group / TILE + r; };
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start(mid) <= id) lo = mid;
+    else hi = mid;
+  }
+  tok0 = first_token(p, lo);
+  const int64_t tok1 = lo == p.requests ? p.tokens : max(first_token(p, lo + 1), tok0);
+  rows = (tok1 - tok0) * p.group;
+  row0 = (id - start(lo)) * TILE;
+  return lo;
+}
+
+__device__ __forceinline__ void store_rowpart(const KvAttnParams& p, int64_t tok, int head, int d, float x) {
+  if (d >= p.c.head_dim) return;
+  const int64_t at = tok * p.o_tok + head * p.o_head + d;
+  if (p.f16) ((_Float16*)p.o)[at] = (_Float16)x;
+  else ((__bf16*)p.o)[at] = (__bf16)x;
+}
+
+// log of a row's sum from its maximum (with the page's exponent) and l.  l's own exponent goes to the maximum first:
+// what the page's scale put into both cancels there exactly.
+__device__ __forceinline__ float row_lse(float top, float l) {
+  if (l == 0.f) return -INFINITY;
+  int x;
+  const float frac = frexpf(l, &x);
+  return kLn2 * ((top + ((float)x - kShift)) + __log2f(frac));
+}
+
+// Few rows: a workgroup has 16 * NQ rows of one key head, its four waves take every fourth 64-key tile straight from
+// memory into registers, and their sums are joined in LDS.  blockIdx.z: a part of the keys.
+template <typename E, int DIM, int NQ>
+__global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
+  constexpr int TILE = 16 * NQ, KS = DIM / 32, DT = DIM / 16, HF = DIM / 64;
+  using vec8 = typename E::vec8;
+  __shared__ float so[4][TILE][DIM + 4];
+  __shared__ float sm[4][TILE], sl[4][TILE];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 15, g = lane >> 4;
+  const int hk = blockIdx.y, z = blockIdx.z;
+  const KvCache& c = p.c;
+  const int page = 1 << c.page_log2;
+
+  int64_t tok0, rows, row0;
+  const int r = find_tile<TILE>(p, blockIdx.x, tok0, rows, row0);
+  if (row0 < 0 || row0 >= rows) return;  // below 0: row starts that do not ascend
+  if (r == p.requests) {  // behind the last request
+    if (p.zero_tail && z == 0 && p.splits == 1)
+      for (int e = tid; e < TILE * DIM; e += 256) {
+        const int64_t i = row0 + e / DIM;
+        if (i >= rows) break;
+        store_rowpart(p, tok0 + i / p.group, hk * p.group + (int)(i % p.group), e % DIM, 0.f);
+        if (e % DIM == 0 && p.lse) p.lse[(tok0 + i / p.group) * p.q_heads + hk * p.group + (int)(i % p.group)] = -INFINITY;
+      }
+    return;
+  }
+  const int64_t n_tok = rows / p.group;
+  const int64_t len = min(min(max((int64_t)p.lens[r], (int64_t)0), p.max_kv), p.width << c.page_log2);
+  const int64_t pos_base = (int64_t)max(p.lens[r], 0) - n_tok;
+  const int32_t* table = p.tables + r * p.table_stride;
+
+  // This lane's rows: what they see is [lo, hi).
+  int64_t qtok[NQ];
+  int qhead[NQ], lo[NQ], hi[NQ];
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    const int64_t i = min(row0 + 16 * t + m, rows - 1);
+    qtok[t] = i / p.group;
+    qhead[t] = hk * p.group + (int)(i - qtok[t] * p.group);
+    const int64_t pos = pos_base + qtok[t];
+    hi[t] = (int)(p.causal ? min(max(pos + 1, (int64_t)0), len) : len);
+    lo[t] = (int)(p.window ? min(max(pos - p.window + 1, (int64_t)0), len) : 0);
+    qtok[t] += tok0;
+  }
+  // What the tile's rows see together, in tiles of 64 keys; this part's share of them.
+  const int64_t last = min(row0 + TILE, rows) - 1;
+  const int64_t pos_first = pos_base + row0 / p.group, pos_last = pos_base + last / p.group;
+  const int khi = (int)(p.causal ? min(max(pos_last + 1, (int64_t)0), len) : len);
+  const int klo = (int)(p.window ? min(max(pos_first - p.window + 1, (int64_t)0), len) : 0);
+  const int tile_lo = klo >> 6, tile_hi = max(tile_lo, (khi + 63) >> 6);
+  const int per = (tile_hi - tile_lo + p.splits - 1) / p.splits;
+  const int tb = min(tile_lo + z * per, tile_hi), te = min(tb + per, tile_hi);
+
+  // q as B operands: channels 64 hf + 16 g + 8 u .. + 7 for k-step 2 hf + u.
+  vec8 qf[NQ][KS];
+#pragma unroll
+  for (int t = 0; t < NQ; ++t)
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d0 = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+      const uint16_t* row = (const uint16_t*)p.q + qtok[t] * p.q_tok + qhead[t] * p.q_head;
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
+      if (p.q_vec && d0 + 8 <= c.head_dim) {
+        const uint4 x = *reinterpret_cast<const uint4*>(row + d0);
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (d0 + e < c.head_dim) w[e >> 1] |= (uint32_t)row[d0 + e] << (16 * (e & 1));
+      }
+      qf[t][s] = as_vec8<E>((u32x4_t){w[0], w[1], w[2], w[3]});
+    }
+
+  f32x4_t o[DT][NQ];
+  float l_run[NQ], m_run[NQ];
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    l_run[t] = 0.f;
+    m_run[t] = -INFINITY;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt][t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  }
+
+  // Page of key j, or -1.
+  auto page_of = [&](int j) -> int {
+    if (j >= len) return -1;
+    const int id = table[j >> c.page_log2];
+    return id >= 0 && id < c.num_pages ? id : -1;
+  };
+  const int64_t page_bytes = (int64_t)page * DIM;
+
+  for (int tile = tb + wave; tile < te; tile += 4) {
+    const int j0 = tile * 64;
+    const int jk = j0 + 16 * (m >> 2), jv = j0 + 16 * g;
+    const int kid = max(page_of(jk), 0), vid = page_of(jv);
+    const bool here = vid >= 0;
+    const int64_t vat = (int64_t)max(vid, 0) * c.heads + hk;
+    const uint8_t* kp = c.k + ((int64_t)kid * c.heads + hk) * page_bytes + ((jk & (page - 1)) + (m & 3)) * DIM + 16 * g;
+    const uint8_t* vp = c.v + vat * page_bytes + m * page + (jv & (page - 1));
+    uint4 kr[4][HF], vr[DT];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int f = 0; f < HF; ++f) kr[t][f] = *reinterpret_cast<const uint4*>(kp + 4 * t * DIM + 64 * f);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) vr[dt] = *reinterpret_cast<const uint4*>(vp + 16 * dt * page);
+    const int ke = min(max((int)c.k_exp[vat], kKvExpMin), kKvExpMax), ve = min(max((int)c.v_exp[vat], kKvExpMin), kKvExpMax);
+
+    f32x4_t s[4][NQ];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) s[t][q] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int f = 0; f < HF; ++f) {
+        const vec8 a0 = widen<E>(kr[t][f].x, kr[t][f].y), a1 = widen<E>(kr[t][f].z, kr[t][f].w);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          s[t][q] = E::mfma16(a0, qf[q][2 * f], s[t][q]);
+          s[t][q] = E::mfma16(a1, qf[q][2 * f + 1], s[t][q]);
+        }
+      }
+
+    // Keys that a row does not see.
+    bool all_seen = here;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) all_seen = all_seen && lo[q] <= jv && jv + 16 <= hi[q];
+    const bool whole = __all(all_seen);
+    bool poison = false;
+    if (!whole) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = jv + 4 * t + i;
+            if (!here || j < lo[q] || j >= hi[q]) s[t][q][i] = -INFINITY;
+          }
+      // Codes behind the last key are whatever the page held: zero times them has to be zero.  A NaN among the
+      // request's own codes must not reach rows that do not see it.
+      const int64_t valid = here ? len - jv : 0;
+      const int nb = (int)min(max(valid, (int64_t)0), (int64_t)16);
+      uint32_t any = 0u;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        vr[dt].x &= first_bytes(nb);
+        vr[dt].y &= first_bytes(nb - 4);
+        vr[dt].z &= first_bytes(nb - 8);
+        vr[dt].w &= first_bytes(nb - 12);
+        any |= nan_bytes(vr[dt].x) | nan_bytes(vr[dt].y) | nan_bytes(vr[dt].z) | nan_bytes(vr[dt].w);
+      }
+      poison = __any(any != 0u);
+    }
+    const float sc = ldexpf(p.scale, ke);
+    f16x8_t pf[2][NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][q][i]);
+      mx = quad16_max(fmaf(mx, sc, (float)ve));
+      if (__any(mx > m_run[q])) {
+        const float m_new = fmaxf(m_run[q], mx);
+        const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run[q] - m_new);
+        m_run[q] = m_new;
+        l_run[q] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[dt][q][i] *= alpha;
+      }
+      const float off = m_run[q] == -INFINITY ? 0.f : (float)ve - m_run[q] + kShift;
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f32x4_t& x = s[2 * u + (e >> 1)][q];
+          const float p0 = fast_exp2(fmaf(x[2 * (e & 1)], sc, off));
+          const float p1 = fast_exp2(fmaf(x[2 * (e & 1) + 1], sc, off));
+          w[e] = F16::pack2(p0, p1);
+          sum += p0 + p1;
+        }
+        pf[u][q] = as_vec8<F16>((u32x4_t){w[0], w[1], w[2], w[3]});
+      }
+      l_run[q] += ldexpf(sum, -ve);
+    }
+    if (poison) {
+      // 1 at each NaN code times 1 at each key that the row sees: rows with a product above 0 are NaN there.
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        uint32_t w[4] = {vr[dt].x, vr[dt].y, vr[dt].z, vr[dt].w};
+        uint32_t ind[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t n = nan_bytes(w[e]);
+          w[e] &= ~(n | (n - (n >> 7)));     // 0xff over each NaN byte
+          ind[e] = (n >> 7) * 0x38u;         // e4m3's 1.0
+        }
+        vr[dt] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          f32x4_t hit = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            f16x8_t seen;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int j = jv + 8 * u + e;
+              seen[e] = (_Float16)(here && j >= lo[q] && j < hi[q] ? 1.f : 0.f);
+            }
+            hit = F16::mfma16(widen_f16(ind[2 * u], ind[2 * u + 1]), seen, hit);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (hit[i] > 0.f) o[dt][q][i] = __uint_as_float(0x7fc00000u);
+        }
+      }
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const f16x8_t a0 = widen_f16(vr[dt].x, vr[dt].y), a1 = widen_f16(vr[dt].z, vr[dt].w);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        o[dt][q] = F16::mfma16(a0, pf[0][q], o[dt][q]);
+        o[dt][q] = F16::mfma16(a1, pf[1][q], o[dt][q]);
+      }
+    }
+  }
+
+  // Join the waves.
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const float l = quad16_sum(l_run[q]);
+    if (g == 0) {
+      sm[wave][16 * q + m] = m_run[q];
+      sl[wave][16 * q + m] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(&so[wave][16 * q + m][16 * dt + 4 * g]) = o[dt][q];
+  }
+  __syncthreads();
+  for (int e = tid; e < TILE * DIM / 4; e += 256) {
+    const int i = e / (DIM / 4), d = (e % (DIM / 4)) * 4;
+    const int64_t row = row0 + i;
+    if (row >= rows) break;
+    const int64_t tok = tok0 + row / p.group;
+    const int head = hk * p.group + (int)(row % p.group);
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w][i]);
+    float l = 0.f;
+    f32x4_t acc = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = sm[w][i] == -INFINITY ? 0.f : fast_exp2(sm[w][i] - top);
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(&so[w][i][d]);
+      l += f * sl[w][i];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += f * x[k];
+    }
+    if (p.splits == 1) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) store_rowpart(p, tok, head, d + k, acc[k] * inv);
+      if (d == 0 && p.lse) p.lse[tok * p.q_heads + head] = row_lse(top, l);
+    } else {
+      const int64_t at = (int64_t)z * p.tokens * p.q_heads + tok * p.q_heads + head;
+      *reinterpret_cast<f32x4_t*>(p.part_o + at * DIM + d) = acc;
+      if (d == 0) {
+        p.part_ml[2 * at] = top;
+        p.part_ml[2 * at + 1] = l;
+      }
+    }
+  }
+}
+
+// Join the parts of the keys: one wave a row.
+template <int DIM>
+__global__ __launch_bounds__(256) void kv_attn_join(KvAttnParams p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t all = p.tokens * p.q_heads;
+  if (row >= all) return;
+  const int64_t tok = row / p.q_heads;
+  const int head = (int)(row - tok * p.q_heads);
+  const bool behind = p.cu_q != nullptr && tok >= min(max((int64_t)p.cu_q[p.requests], (int64_t)0), p.tokens);
+  if (behind && !p.zero_tail) return;
+  constexpr int N = DIM / 64;
+  float top = -INFINITY, l = 0.f, acc[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) acc[k] = 0.f;
+  if (!behind) {
+    for (int z = 0; z < p.splits; ++z) top = fmaxf(top, p.part_ml[2 * (z * all + row)]);
+    for (int z = 0; z < p.splits; ++z) {
+      const float m = p.part_ml[2 * (z * all + row)], lz = p.part_ml[2 * (z * all + row) + 1];
+      if (lz == 0.f) continue;
+      const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);  // m is -inf beside a NaN l where NaN is all that a row sees
+      l += f * lz;
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] += f * p.part_o[(z * all + row) * DIM + N * lane + k];
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int k = 0; k < N; ++k) store_rowpart(p, tok, head, N * lane + k, acc[k] * inv);
+  if (lane == 0 && p.lse) p.lse[row] = row_lse(top, l);
+}
+
+template <typename E, int DIM, int NQ>
+hipError_t launch_rows(const KvAttnParams& p, hipStream_t stream) {
+  const int64_t tiles = p.tokens * p.group / (16 * NQ) + p.requests + 1;
+  if (tiles > 0x7fffffff || p.c.heads > 65535 || p.splits > 65535) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)tiles, (unsigned)p.c.heads, (unsigned)p.splits);
+  hipLaunchKernelGGL((kv_attn_rows<E, DIM, NQ>), grid, dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+template <typename E, int DIM>
+hipError_t launch_any(const KvAttnParams& p, int rows, hipStream_t stream) {
+  hipError_t e = launch_rows<E, DIM, 1>(p, stream);
+  if (e != hipSuccess || p.splits == 1) return e;
+  const int64_t wgs = (p.tokens * p.q_heads + 3) / 4;
+  if (wgs > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(kv_attn_join<DIM>, dim3((unsigned)wgs), dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// Tile and parts of the keys, from the sizes that the host knows.
+KvAttnPlan kv_attn_plan(int64_t tokens, int requests, int q_heads, int kv_heads, int64_t max_kv) {
+  const int group = q_heads / kv_heads;
+  const int64_t mean = (tokens * group + requests - 1) / requests;
+  KvAttnPlan plan;
+  plan.rows = 16;
+  const int64_t wgs = ((tokens * group + plan.rows - 1) / plan.rows + (mean % plan.rows ? requests - 1 : 0)) * kv_heads;
+  // Four tiles a part at least; enough parts for two workgroups on each compute unit.
+  const int64_t most = (max_kv + 255) / 256;
+  int64_t want = (1024 + wgs - 1) / wgs;
+  if (want > most) want = most;
+  if (want > 64) want = 64;
+  if (want < 1) want = 1;
+  plan.splits = (int)want;
+  return plan;
+}
+
+hipError_t launch_kv_attn(const KvAttnParams& p, hipStream_t stream) {
+  const KvAttnPlan plan = kv_attn_plan(p.tokens, p.requests, p.q_heads, p.c.heads, p.max_kv);
+  if (plan.splits != p.splits) return hipErrorInvalidValue;
+  if (p.c.dim == 128) return p.f16 ? launch_any<F16, 128>(p, plan.rows, stream) : launch_any<Bf16, 128>(p, plan.rows, stream);
+  if (p.c.dim == 64) return p.f16 ? launch_any<F16, 64>(p, plan.rows, stream) : launch_any<Bf16, 64>(p, plan.rows, stream);
+  return hipErrorInvalidValue;
+}
+
+}  // namespace pasa
