@@ -4,8 +4,8 @@
 // pos = len - n + i and sees the keys j with j < len, j <= pos if causal, j > pos - window with a window, and a page in
 // the table.  With a page's exponents ke, ve:
 //   s_j = scale 2^ke q.k8_j,   o = sum_j 2^(s_j - m) 2^ve v8_j / sum_j 2^(s_j - m)        (scale holds log2 e)
-// m is the running maximum of s_j + ve, so that p_j = 2^(s_j + ve - m + 15) <= 2^15 carries the page's scale and stays
-// inside fp16's normal numbers down to 2^-29 of the largest; the row sum takes p_j 2^-ve, which is exact.
+// m is a running maximum of s_j + ve (short of it by at most 8), so that p_j = 2^(s_j + ve - m + 7) <= 2^15 carries the
+// page's scale and stays inside fp16's normal numbers down to 2^-21 of 2^m; the row sum takes p_j 2^-ve, which is exact.
 // Rows that see no key get 0, and -inf as the logarithm of their sum.
 //
 // The codes go to the matrix unit as they lie in memory.  Both products contract over what is contiguous in the cache,
@@ -25,7 +25,8 @@ namespace pasa {
 
 namespace {
 
-constexpr float kShift = 15.f;
+constexpr float kShift = 7.f;
+constexpr float kSlack = 8.f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
@@ -100,6 +101,144 @@ __device__ __forceinline__ float row_lse(float top, float l) {
   return kLn2 * ((top + ((float)x - kShift)) + __log2f(frac));
 }
 
+// Rows behind the last request.
+template <int TILE, int DIM>
+__device__ __forceinline__ void zero_rows(const KvAttnParams& p, int hk, int z, int64_t tok0, int64_t rows, int64_t row0) {
+  if (!p.zero_tail || z != 0 || p.splits != 1) return;  // with parts, the join writes them
+  for (int e = threadIdx.x; e < TILE * DIM; e += 256) {
+    const int64_t i = row0 + e / DIM;
+    if (i >= rows) break;
+    const int64_t tok = tok0 + i / p.group;
+    const int head = hk * p.group + (int)(i % p.group);
+    store_rowpart(p, tok, head, e % DIM, 0.f);
+    if (e % DIM == 0 && p.lse) p.lse[tok * p.q_heads + head] = -INFINITY;
+  }
+}
+
+// Four channels from d on, times inv.
+__device__ __forceinline__ void store4(const KvAttnParams& p, int64_t tok, int head, int d, const f32x4_t& x, float inv) {
+  if (p.o_vec && d + 4 <= p.c.head_dim) {
+    uint2 w;
+    if (p.f16) w = make_uint2(F16::pack2(x[0] * inv, x[1] * inv), F16::pack2(x[2] * inv, x[3] * inv));
+    else w = make_uint2(Bf16::pack2(x[0] * inv, x[1] * inv), Bf16::pack2(x[2] * inv, x[3] * inv));
+    *reinterpret_cast<uint2*>((uint16_t*)p.o + tok * p.o_tok + head * p.o_head + d) = w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) store_rowpart(p, tok, head, d + k, x[k] * inv);
+  }
+}
+
+// A row of q as B operands: channels 64 (s / 2) + 16 g + 8 (s % 2) .. + 7 for k-step s.
+template <typename E, int KS>
+__device__ __forceinline__ void load_q(const KvAttnParams& p, int64_t tok, int head, int g, typename E::vec8 (&qf)[KS]) {
+  const uint16_t* row = (const uint16_t*)p.q + tok * p.q_tok + head * p.q_head;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d0 = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    if (p.q_vec && d0 + 8 <= p.c.head_dim) {
+      const uint4 x = *reinterpret_cast<const uint4*>(row + d0);
+      w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (d0 + e < p.c.head_dim) w[e >> 1] |= (uint32_t)row[d0 + e] << (16 * (e & 1));
+    }
+    qf[s] = as_vec8<E>((u32x4_t){w[0], w[1], w[2], w[3]});
+  }
+}
+
+// One tile's online softmax for row tile q: scores s to p as two k-steps of B operands, the running maximum and sum, and
+// o scaled where the maximum rose.  A maximum that rises by less than kSlack is left alone: p then stays below
+// 2^(kShift + kSlack), inside fp16, and a rise that takes the scaling of o's registers is rare.
+template <int DT, int NQ>
+__device__ __forceinline__ void softmax_step(const f32x4_t (&s)[4][NQ], int q, float sc, int ve, float& m_run, float& l_run,
+                                             f32x4_t (&o)[DT][NQ], f16x8_t& p0, f16x8_t& p1) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][q][i]);
+  mx = fmaf(mx, sc, (float)ve);
+  if (__any(mx > m_run + kSlack)) {
+    const float m_new = fmaxf(m_run, quad16_max(mx));
+    const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+    m_run = m_new;
+    l_run *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[dt][q][i] *= alpha;
+  }
+  const float off = m_run == -INFINITY ? 0.f : (float)ve - m_run + kShift;
+  float sum[2] = {0.f, 0.f};
+  uint32_t w[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const f32x4_t& x = s[e >> 1][q];
+    const float a = fast_exp2(fmaf(x[2 * (e & 1)], sc, off));
+    const float b = fast_exp2(fmaf(x[2 * (e & 1) + 1], sc, off));
+    w[e] = F16::pack2(a, b);
+    sum[e & 1] += a + b;
+  }
+  p0 = as_vec8<F16>((u32x4_t){w[0], w[1], w[2], w[3]});
+  p1 = as_vec8<F16>((u32x4_t){w[4], w[5], w[6], w[7]});
+  l_run += ldexpf(sum[0] + sum[1], -ve);
+}
+
+// 0x8000 in each 16-bit half that is an infinity or NaN (among widened codes: NaN).
+__device__ __forceinline__ uint32_t nan_halves(uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
+
+// A tile in LDS that not every row sees whole: a NaN among its values must not reach rows that do not see its key.
+// Where the tile holds one, the outputs that it does reach become NaN: 1 at each NaN times 1 at each key that the row
+// sees is above 0 there.  The products themselves then run on the values without NaN (finite_halves).
+template <int DT>
+__device__ __forceinline__ void poison_step(const unsigned char* vs, int lane, bool here, int jv, const int (&lo)[2], const int (&hi)[2],
+                                            f32x4_t (&o)[DT][2]) {
+  uint32_t any = 0u;
+#pragma unroll 2
+  for (int f = 0; f < 2 * DT; ++f) {
+    const uint4 w = *(reinterpret_cast<const uint4*>(vs + f * 1024) + lane);
+    any |= nan_halves(w.x) | nan_halves(w.y) | nan_halves(w.z) | nan_halves(w.w);
+  }
+  if (!__any(any != 0u)) return;
+  uint64_t hits = 0u;  // bit 8 dt + 4 q + i
+#pragma unroll 1
+  for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      f32x4_t hit = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const f16x8_t a = *(reinterpret_cast<const f16x8_t*>(vs + (2 * dt + u) * 1024) + lane);
+        f16x8_t ind, seen;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = jv + 8 * u + e;
+          ind[e] = (_Float16)(a[e] != a[e] ? 1.f : 0.f);
+          seen[e] = (_Float16)(here && j >= lo[q] && j < hi[q] ? 1.f : 0.f);
+        }
+        hit = F16::mfma16(ind, seen, hit);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (hit[i] > 0.f) hits |= 1ull << (8 * dt + 4 * q + i);
+    }
+  }
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if ((hits >> (8 * dt + 4 * q + i)) & 1u) o[dt][q][i] = __uint_as_float(0x7fc00000u);
+}
+
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
+  const uint32_t n = nan_halves(w);
+  return w & ~(n | (n - (n >> 15)));
+}
+
 // Few rows: a workgroup has 16 * NQ rows of one key head, its four waves take every fourth 64-key tile straight from
 // memory into registers, and their sums are joined in LDS.  blockIdx.z: a part of the keys.
 template <typename E, int DIM, int NQ>
@@ -118,14 +257,8 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
   int64_t tok0, rows, row0;
   const int r = find_tile<TILE>(p, blockIdx.x, tok0, rows, row0);
   if (row0 < 0 || row0 >= rows) return;  // below 0: row starts that do not ascend
-  if (r == p.requests) {  // behind the last request
-    if (p.zero_tail && z == 0 && p.splits == 1)
-      for (int e = tid; e < TILE * DIM; e += 256) {
-        const int64_t i = row0 + e / DIM;
-        if (i >= rows) break;
-        store_rowpart(p, tok0 + i / p.group, hk * p.group + (int)(i % p.group), e % DIM, 0.f);
-        if (e % DIM == 0 && p.lse) p.lse[(tok0 + i / p.group) * p.q_heads + hk * p.group + (int)(i % p.group)] = -INFINITY;
-      }
+  if (r == p.requests) {
+    zero_rows<TILE, DIM>(p, hk, z, tok0, rows, row0);
     return;
   }
   const int64_t n_tok = rows / p.group;
@@ -155,25 +288,9 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
   const int per = (tile_hi - tile_lo + p.splits - 1) / p.splits;
   const int tb = min(tile_lo + z * per, tile_hi), te = min(tb + per, tile_hi);
 
-  // q as B operands: channels 64 hf + 16 g + 8 u .. + 7 for k-step 2 hf + u.
   vec8 qf[NQ][KS];
 #pragma unroll
-  for (int t = 0; t < NQ; ++t)
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d0 = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
-      const uint16_t* row = (const uint16_t*)p.q + qtok[t] * p.q_tok + qhead[t] * p.q_head;
-      uint32_t w[4] = {0u, 0u, 0u, 0u};
-      if (p.q_vec && d0 + 8 <= c.head_dim) {
-        const uint4 x = *reinterpret_cast<const uint4*>(row + d0);
-        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (d0 + e < c.head_dim) w[e >> 1] |= (uint32_t)row[d0 + e] << (16 * (e & 1));
-      }
-      qf[t][s] = as_vec8<E>((u32x4_t){w[0], w[1], w[2], w[3]});
-    }
+  for (int t = 0; t < NQ; ++t) load_q<E, KS>(p, qtok[t], qhead[t], g, qf[t]);
 
   f32x4_t o[DT][NQ];
   float l_run[NQ], m_run[NQ];
@@ -261,40 +378,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
     const float sc = ldexpf(p.scale, ke);
     f16x8_t pf[2][NQ];
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][q][i]);
-      mx = quad16_max(fmaf(mx, sc, (float)ve));
-      if (__any(mx > m_run[q])) {
-        const float m_new = fmaxf(m_run[q], mx);
-        const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run[q] - m_new);
-        m_run[q] = m_new;
-        l_run[q] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[dt][q][i] *= alpha;
-      }
-      const float off = m_run[q] == -INFINITY ? 0.f : (float)ve - m_run[q] + kShift;
-      float sum = 0.f;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const f32x4_t& x = s[2 * u + (e >> 1)][q];
-          const float p0 = fast_exp2(fmaf(x[2 * (e & 1)], sc, off));
-          const float p1 = fast_exp2(fmaf(x[2 * (e & 1) + 1], sc, off));
-          w[e] = F16::pack2(p0, p1);
-          sum += p0 + p1;
-        }
-        pf[u][q] = as_vec8<F16>((u32x4_t){w[0], w[1], w[2], w[3]});
-      }
-      l_run[q] += ldexpf(sum, -ve);
-    }
+    for (int q = 0; q < NQ; ++q) softmax_step<DT, NQ>(s, q, sc, ve, m_run[q], l_run[q], o, pf[0][q], pf[1][q]);
     if (poison) {
       // 1 at each NaN code times 1 at each key that the row sees: rows with a product above 0 are NaN there.
 #pragma unroll
@@ -371,14 +455,225 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
     }
     if (p.splits == 1) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) store_rowpart(p, tok, head, d + k, acc[k] * inv);
+      store4(p, tok, head, d, acc, inv);
       if (d == 0 && p.lse) p.lse[tok * p.q_heads + head] = row_lse(top, l);
     } else {
       const int64_t at = (int64_t)z * p.tokens * p.q_heads + tok * p.q_heads + head;
       *reinterpret_cast<f32x4_t*>(p.part_o + at * DIM + d) = acc;
       if (d == 0) {
         p.part_ml[2 * at] = top;
+        p.part_ml[2 * at + 1] = l;
+      }
+    }
+  }
+}
+
+// ---- many rows --------------------------------------------------------------------
+// A workgroup has 128 rows of one key head, 32 a wave, and walks the keys in tiles of 64.  A tile's codes come from
+// memory once for the workgroup: each thread widens 16-byte pieces and writes them to LDS as the operands that the
+// waves' MFMAs read (1 KB pieces, lane after lane: no bank conflicts either way), while the tile before is computed.
+// Two buffers, one barrier a tile.  Widening once for 128 rows costs 32 conversions a thread and tile of 16-bit LDS
+// traffic; widening after the LDS read would cost each wave 128.
+template <int DIM>
+struct KvTile {
+  static constexpr int ROWS = 128;
+  static constexpr int KS = DIM / 32, DT = DIM / 16, HF = DIM / 64;
+  static constexpr int KBYTES = 64 * DIM * 2, VBYTES = KBYTES;
+};
+
+template <typename E, int DIM>
+__global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int64_t tiles, int64_t items, int64_t per_xcd) {
+  using C = KvTile<DIM>;
+  constexpr int KS = C::KS, DT = C::DT, HF = C::HF;
+  using vec8 = typename E::vec8;
+  __shared__ __attribute__((aligned(1024))) unsigned char Ks[2][C::KBYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char Vs[2][C::VBYTES];
+  // Workgroup n runs on XCD n % 8, which takes a contiguous run of (head, part of the keys, tile): the tiles of a
+  // head sweep the same keys at the same time and find them in the XCD's L2.
+  const int64_t item = (int64_t)(blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if ((int64_t)(blockIdx.x >> 3) >= per_xcd || item >= items) return;
+  const int hk = (int)(item / (tiles * p.splits));
+  const int z = (int)(item / tiles % p.splits);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 15, g = lane >> 4;
+  const KvCache& c = p.c;
+  const int page = 1 << c.page_log2;
+
+  int64_t tok0, rows, row0;
+  const int r = find_tile<C::ROWS>(p, item % tiles, tok0, rows, row0);
+  if (row0 < 0 || row0 >= rows) return;
+  if (r == p.requests) {
+    zero_rows<C::ROWS, DIM>(p, hk, z, tok0, rows, row0);
+    return;
+  }
+  const int64_t n_tok = rows / p.group;
+  const int64_t len64 = min(min(max((int64_t)p.lens[r], (int64_t)0), p.max_kv), p.width << c.page_log2);
+  const int len = (int)len64;
+  const int64_t pos_base = (int64_t)max(p.lens[r], 0) - n_tok;
+  const int32_t* table = p.tables + r * p.table_stride;
+  auto sees_lo = [&](int64_t pos) { return (int)(p.window ? min(max(pos - p.window + 1, (int64_t)0), len64) : 0); };
+  auto sees_hi = [&](int64_t pos) { return (int)(p.causal ? min(max(pos + 1, (int64_t)0), len64) : len64); };
+
+  // This lane's two rows, and what they see: [lo, hi).
+  const int64_t wrow = row0 + 32 * wave;
+  int64_t qtok[2];
+  int qhead[2], lo[2], hi[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int64_t i = min(wrow + 16 * q + m, rows - 1);
+    qtok[q] = i / p.group;
+    qhead[q] = hk * p.group + (int)(i - qtok[q] * p.group);
+    lo[q] = sees_lo(pos_base + qtok[q]);
+    hi[q] = sees_hi(pos_base + qtok[q]);
+    qtok[q] += tok0;
+  }
+  const int64_t last = min(row0 + C::ROWS, rows) - 1;
+  const int khi = sees_hi(pos_base + last / p.group), klo = sees_lo(pos_base + row0 / p.group);
+  // Keys that every row of the wave sees.
+  const int w_lo = sees_lo(pos_base + min(wrow + 31, rows - 1) / p.group), w_hi = sees_hi(pos_base + min(wrow, rows - 1) / p.group);
+  const int tile_lo = klo >> 6, tile_hi = max(tile_lo, (khi + 63) >> 6);
+  const int per = (tile_hi - tile_lo + p.splits - 1) / p.splits;
+  const int tb = min(tile_lo + z * per, tile_hi), te = min(tb + per, tile_hi);
+
+  vec8 qf[2][KS];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) load_q<E, KS>(p, qtok[q], qhead[q], g, qf[q]);
+
+  f32x4_t o[DT][2];
+  float l_run[2] = {0.f, 0.f}, m_run[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt][q] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+
+  auto page_of = [&](int j) -> int {
+    if (j >= len) return -1;
+    const int id = table[j >> c.page_log2];
+    return id >= 0 && id < c.num_pages ? id : -1;
+  };
+  const int64_t page_bytes = (int64_t)page * DIM;
+  // Pieces of a tile that this thread brings: of 16-key tile `wave` of K row m's 16 channels 64 f + 16 g .. of each
+  // f; of V channels 16 (HF wave + f) + m, keys 16 g .. + 15.
+  uint4 kr[HF], vr[HF];
+  int kid = -1, vid = -1;        // pages of the next tile's pieces
+  int ke_n = 0, ve_n = 0;        // exponents of the next tile (keys 16 g ..)
+  bool here_n = false;
+  auto look_up = [&](int tile) {
+    kid = page_of(tile * 64 + 16 * (m >> 2));
+    vid = page_of(tile * 64 + 16 * g);
+  };
+  auto fetch = [&](int tile) {
+    const int jk = tile * 64 + 16 * (m >> 2), jv = tile * 64 + 16 * g;
+    const uint8_t* kp = c.k + ((int64_t)max(kid, 0) * c.heads + hk) * page_bytes + ((jk & (page - 1)) + 4 * wave + (m & 3)) * DIM + 16 * g;
+    const int64_t at = (int64_t)max(vid, 0) * c.heads + hk;
+    const uint8_t* vp = c.v + at * page_bytes + (16 * HF * wave + m) * page + (jv & (page - 1));
+#pragma unroll
+    for (int f = 0; f < HF; ++f) {
+      kr[f] = *reinterpret_cast<const uint4*>(kp + 64 * f);
+      vr[f] = *reinterpret_cast<const uint4*>(vp + 16 * f * page);
+    }
+    ke_n = c.k_exp[at];
+    ve_n = c.v_exp[at];
+    here_n = vid >= 0;
+  };
+  auto stage = [&](int tile, int b) {
+    if (tile * 64 + 64 > len || !__all(here_n)) {  // codes behind the last key are whatever the page held
+      const int nb = here_n ? min(max(len - tile * 64 - 16 * g, 0), 16) : 0;
+#pragma unroll
+      for (int f = 0; f < HF; ++f)
+        vr[f] = make_uint4(vr[f].x & first_bytes(nb), vr[f].y & first_bytes(nb - 4), vr[f].z & first_bytes(nb - 8), vr[f].w & first_bytes(nb - 12));
+    }
+#pragma unroll
+    for (int f = 0; f < HF; ++f) {
+      vec8* kd = reinterpret_cast<vec8*>(Ks[b] + (wave * KS + 2 * f) * 1024) + lane;
+      kd[0] = widen<E>(kr[f].x, kr[f].y);
+      kd[64] = widen<E>(kr[f].z, kr[f].w);
+      f16x8_t* vd = reinterpret_cast<f16x8_t*>(Vs[b] + (HF * wave + f) * 2048) + lane;
+      vd[0] = widen_f16(vr[f].x, vr[f].y);
+      vd[64] = widen_f16(vr[f].z, vr[f].w);
+    }
+  };
+
+  if (tb < te) {
+    look_up(tb);
+    fetch(tb);
+    if (tb + 1 < te) look_up(tb + 1);
+    stage(tb, 0);
+  }
+  for (int tile = tb; tile < te; ++tile) {
+    const int b = (tile - tb) & 1;
+    const int ke = min(max(ke_n, kKvExpMin), kKvExpMax), ve = min(max(ve_n, kKvExpMin), kKvExpMax);
+    const bool here = here_n;
+    barrier_lds_reads_done();  // this tile is in LDS, and the other buffer is no longer read
+    if (tile + 1 < te) {
+      fetch(tile + 1);
+      if (tile + 2 < te) look_up(tile + 2);
+    }
+    f32x4_t s[4][2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) s[t][q] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const vec8 a = *(reinterpret_cast<const vec8*>(Ks[b] + (t * KS + k) * 1024) + lane);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) s[t][q] = E::mfma16(a, qf[q][k], s[t][q]);
+      }
+    const int j0 = tile * 64, jv = j0 + 16 * g;
+    const bool whole = j0 >= w_lo && j0 + 64 <= w_hi && __all(here);
+    if (!whole) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = jv + 4 * t + i;
+            if (!here || j < lo[q] || j >= hi[q]) s[t][q][i] = -INFINITY;
+          }
+    }
+    const float sc = ldexpf(p.scale, ke);
+    f16x8_t pf[2][2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) softmax_step<DT, 2>(s, q, sc, ve, m_run[q], l_run[q], o, pf[0][q], pf[1][q]);
+    auto pv = [&](auto fix) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const f16x8_t a = as_vec8<F16>(fix(*(reinterpret_cast<const uint4*>(Vs[b] + (2 * dt + u) * 1024) + lane)));
+#pragma unroll
+          for (int q = 0; q < 2; ++q) o[dt][q] = F16::mfma16(a, pf[u][q], o[dt][q]);
+        }
+    };
+    if (whole) {
+      pv([](const uint4& w) { return w; });
+    } else {
+      poison_step<DT>(Vs[b], lane, here, jv, lo, hi, o);
+      pv([](const uint4& w) { return make_uint4(finite_halves(w.x), finite_halves(w.y), finite_halves(w.z), finite_halves(w.w)); });
+    }
+    if (tile + 1 < te) stage(tile + 1, b ^ 1);
+  }
+
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const float l = quad16_sum(l_run[q]);
+    if (wrow + 16 * q + m >= rows) continue;
+    if (p.splits == 1) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) store4(p, qtok[q], qhead[q], 16 * dt + 4 * g, o[dt][q], inv);
+      if (g == 0 && p.lse) p.lse[qtok[q] * p.q_heads + qhead[q]] = row_lse(m_run[q], l);
+    } else {
+      const int64_t at = (int64_t)z * p.tokens * p.q_heads + qtok[q] * p.q_heads + qhead[q];
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(p.part_o + at * DIM + 16 * dt + 4 * g) = o[dt][q];
+      if (g == 0) {
+        p.part_ml[2 * at] = m_run[q];
         p.part_ml[2 * at + 1] = l;
       }
     }
@@ -427,8 +722,18 @@ hipError_t launch_rows(const KvAttnParams& p, hipStream_t stream) {
 }
 
 template <typename E, int DIM>
+hipError_t launch_tiles(const KvAttnParams& p, hipStream_t stream) {
+  const int64_t tiles = p.tokens * p.group / KvTile<DIM>::ROWS + p.requests + 1;
+  const int64_t items = tiles * p.c.heads * p.splits;
+  const int64_t per_xcd = (items + 7) / 8;
+  if (per_xcd * 8 > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((kv_attn_tiles<E, DIM>), dim3((unsigned)(per_xcd * 8)), dim3(256), 0, stream, p, tiles, items, per_xcd);
+  return hipGetLastError();
+}
+
+template <typename E, int DIM>
 hipError_t launch_any(const KvAttnParams& p, int rows, hipStream_t stream) {
-  hipError_t e = launch_rows<E, DIM, 1>(p, stream);
+  const hipError_t e = rows == 16 ? launch_rows<E, DIM, 1>(p, stream) : launch_tiles<E, DIM>(p, stream);
   if (e != hipSuccess || p.splits == 1) return e;
   const int64_t wgs = (p.tokens * p.q_heads + 3) / 4;
   if (wgs > 0x7fffffff) return hipErrorInvalidValue;
@@ -443,11 +748,11 @@ KvAttnPlan kv_attn_plan(int64_t tokens, int requests, int q_heads, int kv_heads,
   const int group = q_heads / kv_heads;
   const int64_t mean = (tokens * group + requests - 1) / requests;
   KvAttnPlan plan;
-  plan.rows = 16;
+  plan.rows = mean <= 16 ? 16 : 128;
   const int64_t wgs = ((tokens * group + plan.rows - 1) / plan.rows + (mean % plan.rows ? requests - 1 : 0)) * kv_heads;
   // Four tiles a part at least; enough parts for two workgroups on each compute unit.
   const int64_t most = (max_kv + 255) / 256;
-  int64_t want = (1024 + wgs - 1) / wgs;
+  int64_t want = ((plan.rows == 16 ? 1024 : 512) + wgs - 1) / wgs;
   if (want > most) want = most;
   if (want > 64) want = 64;
   if (want < 1) want = 1;
