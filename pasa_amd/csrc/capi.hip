@@ -1039,7 +1039,7 @@ static int check_kv8_attn_sizes(int64_t tokens, int64_t requests, int64_t q_head
 size_t pasa_kv8_attn_workspace_bytes(int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t dim,
                                      int64_t max_kv) {
   if (check_kv8_attn_sizes(tokens, requests, q_heads, kv_heads, max_kv) || tokens == 0) return 0;
-  const pasa::KvAttnPlan plan = pasa::kv_attn_plan(tokens, (int)requests, (int)q_heads, (int)kv_heads, max_kv);
+  const pasa::KvAttnPlan plan = pasa::kv_attn_plan(tokens, (int)requests, (int)q_heads, (int)kv_heads, (int)dim, max_kv);
   return plan.splits == 1 ? 0 : (size_t)plan.splits * (size_t)(tokens * q_heads) * (size_t)(dim + 2) * sizeof(float);
 }
 
@@ -1064,7 +1064,7 @@ int pasa_kv8_attn(const pasa_kv8_t* cache, const pasa_kv8_attn_t* a, void* works
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(PASA_ERR_WORKSPACE, "pasa_kv8_attn: workspace %zu bytes < %zu", workspace ? workspace_bytes : (size_t)0, need);
   if (need > 0 && ((uintptr_t)workspace & 15u)) return fail(PASA_ERR_BAD_ARG, "pasa_kv8_attn: workspace must be 16-byte aligned");
-  const pasa::KvAttnPlan plan = pasa::kv_attn_plan(a->tokens, (int)a->requests, (int)a->q_heads, (int)cache->heads, a->max_kv);
+  const pasa::KvAttnPlan plan = pasa::kv_attn_plan(a->tokens, (int)a->requests, (int)a->q_heads, (int)cache->heads, (int)cache->dim, a->max_kv);
   p.q = a->q;
   p.o = a->o;
   p.lse = a->lse;
@@ -1079,6 +1079,7 @@ int pasa_kv8_attn(const pasa_kv8_t* cache, const pasa_kv8_attn_t* a, void* works
   p.cu_q = a->cu_q;
   p.requests = (int)a->requests;
   p.tokens = a->tokens;
+  p.per_request = (int)(a->tokens / a->requests);
   p.q_heads = (int)a->q_heads;
   p.group = (int)(a->q_heads / cache->heads);
   p.max_kv = a->max_kv;

@@ -16,6 +16,8 @@
 //                 keys 16 g .. 16 g + 15 of row m of q: one page, one pair of exponents
 //   O^T += V^T P^T  A row m of 16-channel tile dt is channel 16 dt + m, k-slots keys 16 g + 8 u .. + 7 of step u:
 //                 the lane's own results as they stand, and 16 bytes of V
+#include <math.h>
+
 #include <type_traits>
 
 #include "common.h"
@@ -61,16 +63,17 @@ __device__ __forceinline__ uint32_t first_bytes(int n) {
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 // The requests' first rows of q, clamped to the rows that there are.
-__device__ __forceinline__ int64_t first_token(const KvAttnParams& p, int r) {
-  if (p.cu_q == nullptr) return (int64_t)r * (p.tokens / p.requests);
-  return min(max((int64_t)p.cu_q[r], (int64_t)0), p.tokens);
+// (tokens * q_heads < 2^31: row numbers fit 32 bits.)
+__device__ __forceinline__ int first_token(const KvAttnParams& p, int r) {
+  if (p.cu_q == nullptr) return r * p.per_request;
+  return min(max(p.cu_q[r], 0), (int)p.tokens);
 }
 
 // Tile `id` of the launch: request r (requests: the rows behind the last one), and its first row.  The tiles of a
 // request are numbered from floor(first row / TILE) + r, which leaves room for every request's last, part-filled one
 // without a sum over the requests before it.
 template <int TILE>
-__device__ __forceinline__ int find_tile(const KvAttnParams& p, int64_t id, int64_t& tok0, int64_t& rows, int64_t& row0) {
+__device__ __forceinline__ int find_tile(const KvAttnParams& p, int id, int& tok0, int& rows, int& row0) {
   int lo = 0, hi = p.requests + 1;
   auto start = [&](int r) { return first_token(p, r) * p.group / TILE + r; };
   while (hi - lo > 1) {
@@ -79,10 +82,18 @@ __device__ __forceinline__ int find_tile(const KvAttnParams& p, int64_t id, int6
     else hi = mid;
   }
   tok0 = first_token(p, lo);
-  const int64_t tok1 = lo == p.requests ? p.tokens : max(first_token(p, lo + 1), tok0);
+  const int tok1 = lo == p.requests ? (int)p.tokens : max(first_token(p, lo + 1), tok0);
   rows = (tok1 - tok0) * p.group;
   row0 = (id - start(lo)) * TILE;
   return lo;
+}
+
+// What position pos of a request of len keys sees: [sees_lo, sees_hi).
+__device__ __forceinline__ int sees_lo(const KvAttnParams& p, int64_t pos, int len) {
+  return p.window ? (int)min(max(pos - p.window + 1, (int64_t)0), (int64_t)len) : 0;
+}
+__device__ __forceinline__ int sees_hi(const KvAttnParams& p, int64_t pos, int len) {
+  return p.causal ? (int)min(max(pos + 1, (int64_t)0), (int64_t)len) : len;
 }
 
 __device__ __forceinline__ void store_rowpart(const KvAttnParams& p, int64_t tok, int head, int d, float x) {
@@ -103,13 +114,13 @@ __device__ __forceinline__ float row_lse(float top, float l) {
 
 // Rows behind the last request.
 template <int TILE, int DIM>
-__device__ __forceinline__ void zero_rows(const KvAttnParams& p, int hk, int z, int64_t tok0, int64_t rows, int64_t row0) {
+__device__ __forceinline__ void zero_rows(const KvAttnParams& p, int hk, int z, int tok0, int rows, int row0) {
   if (!p.zero_tail || z != 0 || p.splits != 1) return;  // with parts, the join writes them
   for (int e = threadIdx.x; e < TILE * DIM; e += 256) {
-    const int64_t i = row0 + e / DIM;
+    const int i = row0 + e / DIM;
     if (i >= rows) break;
     const int64_t tok = tok0 + i / p.group;
-    const int head = hk * p.group + (int)(i % p.group);
+    const int head = hk * p.group + i % p.group;
     store_rowpart(p, tok, head, e % DIM, 0.f);
     if (e % DIM == 0 && p.lse) p.lse[tok * p.q_heads + head] = -INFINITY;
   }
@@ -148,18 +159,19 @@ __device__ __forceinline__ void load_q(const KvAttnParams& p, int64_t tok, int h
   }
 }
 
-// One tile's online softmax for row tile q: scores s to p as two k-steps of B operands, the running maximum and sum, and
-// o scaled where the maximum rose.  A maximum that rises by less than kSlack is left alone: p then stays below
-// 2^(kShift + kSlack), inside fp16, and a rise that takes the scaling of o's registers is rare.
+// The largest of a lane's scores of row tile q, with the page's scales.
+template <int NQ>
+__device__ __forceinline__ float lane_max(const f32x4_t (&s)[4][NQ], int q, float sc, float ve) {
+  float mx = fmaxf(s[0][q][0], s[0][q][1]);
+#pragma unroll
+  for (int e = 2; e < 16; e += 2) mx = fmaxf(fmaxf(s[e >> 2][q][e & 3], s[e >> 2][q][(e & 3) + 1]), mx);
+  return fmaf(mx, sc, ve);
+}
+
+// The running maximum of row tile q, and o and l scaled where it rose.  A rise by less than kSlack is left alone: p then
+// stays below 2^(kShift + kSlack), inside fp16, and scaling o's registers is rare.
 template <int DT, int NQ>
-__device__ __forceinline__ void softmax_step(const f32x4_t (&s)[4][NQ], int q, float sc, int ve, float& m_run, float& l_run,
-                                             f32x4_t (&o)[DT][NQ], f16x8_t& p0, f16x8_t& p1) {
-  float mx = -INFINITY;
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][q][i]);
-  mx = fmaf(mx, sc, (float)ve);
+__device__ __forceinline__ void raise_max(float mx, int q, float& m_run, float& l_run, f32x4_t (&o)[DT][NQ]) {
   if (__any(mx > m_run + kSlack)) {
     const float m_new = fmaxf(m_run, quad16_max(mx));
     const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
@@ -170,7 +182,13 @@ __device__ __forceinline__ void softmax_step(const f32x4_t (&s)[4][NQ], int q, f
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[dt][q][i] *= alpha;
   }
-  const float off = m_run == -INFINITY ? 0.f : (float)ve - m_run + kShift;
+}
+
+// Scores of row tile q to p, as two k-steps of B operands, and their sum to l (inv: 2^-ve).
+template <int NQ>
+__device__ __forceinline__ void weights(const f32x4_t (&s)[4][NQ], int q, float sc, float ve, float inv, float m_run, float& l_run,
+                                        f16x8_t& p0, f16x8_t& p1) {
+  const float off = m_run == -INFINITY ? 0.f : ve - m_run + kShift;
   float sum[2] = {0.f, 0.f};
   uint32_t w[8];
 #pragma unroll
@@ -179,12 +197,16 @@ __device__ __forceinline__ void softmax_step(const f32x4_t (&s)[4][NQ], int q, f
     const float a = fast_exp2(fmaf(x[2 * (e & 1)], sc, off));
     const float b = fast_exp2(fmaf(x[2 * (e & 1) + 1], sc, off));
     w[e] = F16::pack2(a, b);
-    sum[e & 1] += a + b;
+    sum[0] += a;
+    sum[1] += b;
   }
   p0 = as_vec8<F16>((u32x4_t){w[0], w[1], w[2], w[3]});
   p1 = as_vec8<F16>((u32x4_t){w[4], w[5], w[6], w[7]});
-  l_run += ldexpf(sum[0] + sum[1], -ve);
+  l_run = fmaf(sum[0] + sum[1], inv, l_run);
 }
+
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+__device__ __forceinline__ int page_exp(int e) { return min(max(e, kKvExpMin), kKvExpMax); }
 
 // 0x8000 in each 16-bit half that is an infinity or NaN (among widened codes: NaN).
 __device__ __forceinline__ uint32_t nan_halves(uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
@@ -254,16 +276,16 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
   const KvCache& c = p.c;
   const int page = 1 << c.page_log2;
 
-  int64_t tok0, rows, row0;
+  int tok0, rows, row0;
   const int r = find_tile<TILE>(p, blockIdx.x, tok0, rows, row0);
   if (row0 < 0 || row0 >= rows) return;  // below 0: row starts that do not ascend
   if (r == p.requests) {
     zero_rows<TILE, DIM>(p, hk, z, tok0, rows, row0);
     return;
   }
-  const int64_t n_tok = rows / p.group;
-  const int64_t len = min(min(max((int64_t)p.lens[r], (int64_t)0), p.max_kv), p.width << c.page_log2);
-  const int64_t pos_base = (int64_t)max(p.lens[r], 0) - n_tok;
+  const int raw_len = max(p.lens[r], 0);
+  const int len = (int)min(min((int64_t)raw_len, p.max_kv), p.width << c.page_log2);
+  const int64_t pos_base = (int64_t)raw_len - rows / p.group;
   const int32_t* table = p.tables + r * p.table_stride;
 
   // This lane's rows: what they see is [lo, hi).
@@ -271,19 +293,15 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
   int qhead[NQ], lo[NQ], hi[NQ];
 #pragma unroll
   for (int t = 0; t < NQ; ++t) {
-    const int64_t i = min(row0 + 16 * t + m, rows - 1);
-    qtok[t] = i / p.group;
-    qhead[t] = hk * p.group + (int)(i - qtok[t] * p.group);
-    const int64_t pos = pos_base + qtok[t];
-    hi[t] = (int)(p.causal ? min(max(pos + 1, (int64_t)0), len) : len);
-    lo[t] = (int)(p.window ? min(max(pos - p.window + 1, (int64_t)0), len) : 0);
-    qtok[t] += tok0;
+    const int i = min(row0 + 16 * t + m, rows - 1), tok = i / p.group;
+    qhead[t] = hk * p.group + (i - tok * p.group);
+    lo[t] = sees_lo(p, pos_base + tok, len);
+    hi[t] = sees_hi(p, pos_base + tok, len);
+    qtok[t] = tok0 + tok;
   }
   // What the tile's rows see together, in tiles of 64 keys; this part's share of them.
-  const int64_t last = min(row0 + TILE, rows) - 1;
-  const int64_t pos_first = pos_base + row0 / p.group, pos_last = pos_base + last / p.group;
-  const int khi = (int)(p.causal ? min(max(pos_last + 1, (int64_t)0), len) : len);
-  const int klo = (int)(p.window ? min(max(pos_first - p.window + 1, (int64_t)0), len) : 0);
+  const int last = min(row0 + TILE, rows) - 1;
+  const int klo = sees_lo(p, pos_base + row0 / p.group, len), khi = sees_hi(p, pos_base + last / p.group, len);
   const int tile_lo = klo >> 6, tile_hi = max(tile_lo, (khi + 63) >> 6);
   const int per = (tile_hi - tile_lo + p.splits - 1) / p.splits;
   const int tb = min(tile_lo + z * per, tile_hi), te = min(tb + per, tile_hi);
@@ -325,7 +343,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
       for (int f = 0; f < HF; ++f) kr[t][f] = *reinterpret_cast<const uint4*>(kp + 4 * t * DIM + 64 * f);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) vr[dt] = *reinterpret_cast<const uint4*>(vp + 16 * dt * page);
-    const int ke = min(max((int)c.k_exp[vat], kKvExpMin), kKvExpMax), ve = min(max((int)c.v_exp[vat], kKvExpMin), kKvExpMax);
+    const int ke = page_exp(c.k_exp[vat]), ve = page_exp(c.v_exp[vat]);
 
     f32x4_t s[4][NQ];
 #pragma unroll
@@ -362,8 +380,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
           }
       // Codes behind the last key are whatever the page held: zero times them has to be zero.  A NaN among the
       // request's own codes must not reach rows that do not see it.
-      const int64_t valid = here ? len - jv : 0;
-      const int nb = (int)min(max(valid, (int64_t)0), (int64_t)16);
+      const int nb = here ? min(max(len - jv, 0), 16) : 0;
       uint32_t any = 0u;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
@@ -375,10 +392,13 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
       }
       poison = __any(any != 0u);
     }
-    const float sc = ldexpf(p.scale, ke);
+    const float sc = p.scale * exp2_int(ke), inv = exp2_int(-ve);
     f16x8_t pf[2][NQ];
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) softmax_step<DT, NQ>(s, q, sc, ve, m_run[q], l_run[q], o, pf[0][q], pf[1][q]);
+    for (int q = 0; q < NQ; ++q) {
+      raise_max<DT, NQ>(lane_max<NQ>(s, q, sc, (float)ve), q, m_run[q], l_run[q], o);
+      weights<NQ>(s, q, sc, (float)ve, inv, m_run[q], l_run[q], pf[0][q], pf[1][q]);
+    }
     if (poison) {
       // 1 at each NaN code times 1 at each key that the row sees: rows with a product above 0 are NaN there.
 #pragma unroll
@@ -436,10 +456,10 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
   __syncthreads();
   for (int e = tid; e < TILE * DIM / 4; e += 256) {
     const int i = e / (DIM / 4), d = (e % (DIM / 4)) * 4;
-    const int64_t row = row0 + i;
+    const int row = row0 + i;
     if (row >= rows) break;
     const int64_t tok = tok0 + row / p.group;
-    const int head = hk * p.group + (int)(row % p.group);
+    const int head = hk * p.group + row % p.group;
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w][i]);
@@ -481,8 +501,11 @@ struct KvTile {
   static constexpr int KBYTES = 64 * DIM * 2, VBYTES = KBYTES;
 };
 
-template <typename E, int DIM>
-__global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int64_t tiles, int64_t items, int64_t per_xcd) {
+constexpr int kAhead = 4;  // LDS reads in flight
+
+// UNI: pages of 64 tokens and more, so that a tile has one page and its number stays in scalar registers.
+template <typename E, int DIM, bool UNI>
+__global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int tiles, int items, int per_xcd) {
   using C = KvTile<DIM>;
   constexpr int KS = C::KS, DT = C::DT, HF = C::HF;
   using vec8 = typename E::vec8;
@@ -490,55 +513,47 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int64_t 
   __shared__ __attribute__((aligned(1024))) unsigned char Vs[2][C::VBYTES];
   // Workgroup n runs on XCD n % 8, which takes a contiguous run of (head, part of the keys, tile): the tiles of a
   // head sweep the same keys at the same time and find them in the XCD's L2.
-  const int64_t item = (int64_t)(blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if ((int64_t)(blockIdx.x >> 3) >= per_xcd || item >= items) return;
-  const int hk = (int)(item / (tiles * p.splits));
-  const int z = (int)(item / tiles % p.splits);
+  const int slot = blockIdx.x >> 3, item = (blockIdx.x & 7) * per_xcd + slot;
+  if (item >= items) return;
+  const int hz = item / tiles, hk = hz / p.splits, z = hz - hk * p.splits;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, g = lane >> 4;
   const KvCache& c = p.c;
   const int page = 1 << c.page_log2;
 
-  int64_t tok0, rows, row0;
-  const int r = find_tile<C::ROWS>(p, item % tiles, tok0, rows, row0);
+  int tok0, rows, row0;
+  const int r = find_tile<C::ROWS>(p, item - hz * tiles, tok0, rows, row0);
   if (row0 < 0 || row0 >= rows) return;
   if (r == p.requests) {
     zero_rows<C::ROWS, DIM>(p, hk, z, tok0, rows, row0);
     return;
   }
-  const int64_t n_tok = rows / p.group;
-  const int64_t len64 = min(min(max((int64_t)p.lens[r], (int64_t)0), p.max_kv), p.width << c.page_log2);
-  const int len = (int)len64;
-  const int64_t pos_base = (int64_t)max(p.lens[r], 0) - n_tok;
+  const int raw_len = max(p.lens[r], 0);
+  const int len = (int)min(min((int64_t)raw_len, p.max_kv), p.width << c.page_log2);
+  const int64_t pos_base = (int64_t)raw_len - rows / p.group;
   const int32_t* table = p.tables + r * p.table_stride;
-  auto sees_lo = [&](int64_t pos) { return (int)(p.window ? min(max(pos - p.window + 1, (int64_t)0), len64) : 0); };
-  auto sees_hi = [&](int64_t pos) { return (int)(p.causal ? min(max(pos + 1, (int64_t)0), len64) : len64); };
 
-  // This lane's two rows, and what they see: [lo, hi).
-  const int64_t wrow = row0 + 32 * wave;
-  int64_t qtok[2];
-  int qhead[2], lo[2], hi[2];
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int64_t i = min(wrow + 16 * q + m, rows - 1);
-    qtok[q] = i / p.group;
-    qhead[q] = hk * p.group + (int)(i - qtok[q] * p.group);
-    lo[q] = sees_lo(pos_base + qtok[q]);
-    hi[q] = sees_hi(pos_base + qtok[q]);
-    qtok[q] += tok0;
-  }
-  const int64_t last = min(row0 + C::ROWS, rows) - 1;
-  const int khi = sees_hi(pos_base + last / p.group), klo = sees_lo(pos_base + row0 / p.group);
-  // Keys that every row of the wave sees.
-  const int w_lo = sees_lo(pos_base + min(wrow + 31, rows - 1) / p.group), w_hi = sees_hi(pos_base + min(wrow, rows - 1) / p.group);
+  // This lane's row of row tile q: its token within the request, and its head.
+  const int wrow = row0 + 32 * wave;
+  auto row_of = [&](int q, int& tok, int& head) {
+    const int i = min(wrow + 16 * q + m, rows - 1);
+    tok = i / p.group;
+    head = hk * p.group + (i - tok * p.group);
+  };
+  const int last = min(row0 + C::ROWS, rows) - 1;
+  const int klo = sees_lo(p, pos_base + row0 / p.group, len), khi = sees_hi(p, pos_base + last / p.group, len);
   const int tile_lo = klo >> 6, tile_hi = max(tile_lo, (khi + 63) >> 6);
   const int per = (tile_hi - tile_lo + p.splits - 1) / p.splits;
   const int tb = min(tile_lo + z * per, tile_hi), te = min(tb + per, tile_hi);
 
   vec8 qf[2][KS];
 #pragma unroll
-  for (int q = 0; q < 2; ++q) load_q<E, KS>(p, qtok[q], qhead[q], g, qf[q]);
+  for (int q = 0; q < 2; ++q) {
+    int tok, head;
+    row_of(q, tok, head);
+    load_q<E, KS>(p, tok0 + tok, head, g, qf[q]);
+  }
 
   f32x4_t o[DT][2];
   float l_run[2] = {0.f, 0.f}, m_run[2] = {-INFINITY, -INFINITY};
@@ -547,70 +562,56 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int64_t 
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt][q] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 
-  auto page_of = [&](int j) -> int {
-    if (j >= len) return -1;
-    const int id = table[j >> c.page_log2];
-    return id >= 0 && id < c.num_pages ? id : -1;
-  };
-  const int64_t page_bytes = (int64_t)page * DIM;
-  // Pieces of a tile that this thread brings: of 16-key tile `wave` of K row m's 16 channels 64 f + 16 g .. of each
-  // f; of V channels 16 (HF wave + f) + m, keys 16 g .. + 15.
-  uint4 kr[HF], vr[HF];
-  int kid = -1, vid = -1;        // pages of the next tile's pieces
-  int ke_n = 0, ve_n = 0;        // exponents of the next tile (keys 16 g ..)
-  bool here_n = false;
-  auto look_up = [&](int tile) {
-    kid = page_of(tile * 64 + 16 * (m >> 2));
-    vid = page_of(tile * 64 + 16 * g);
-  };
-  auto fetch = [&](int tile) {
-    const int jk = tile * 64 + 16 * (m >> 2), jv = tile * 64 + 16 * g;
-    const uint8_t* kp = c.k + ((int64_t)max(kid, 0) * c.heads + hk) * page_bytes + ((jk & (page - 1)) + 4 * wave + (m & 3)) * DIM + 16 * g;
-    const int64_t at = (int64_t)max(vid, 0) * c.heads + hk;
-    const uint8_t* vp = c.v + at * page_bytes + (16 * HF * wave + m) * page + (jv & (page - 1));
-#pragma unroll
-    for (int f = 0; f < HF; ++f) {
-      kr[f] = *reinterpret_cast<const uint4*>(kp + 64 * f);
-      vr[f] = *reinterpret_cast<const uint4*>(vp + 16 * f * page);
-    }
-    ke_n = c.k_exp[at];
-    ve_n = c.v_exp[at];
-    here_n = vid >= 0;
-  };
-  auto stage = [&](int tile, int b) {
-    if (tile * 64 + 64 > len || !__all(here_n)) {  // codes behind the last key are whatever the page held
-      const int nb = here_n ? min(max(len - tile * 64 - 16 * g, 0), 16) : 0;
-#pragma unroll
-      for (int f = 0; f < HF; ++f)
-        vr[f] = make_uint4(vr[f].x & first_bytes(nb), vr[f].y & first_bytes(nb - 4), vr[f].z & first_bytes(nb - 8), vr[f].w & first_bytes(nb - 12));
-    }
-#pragma unroll
-    for (int f = 0; f < HF; ++f) {
-      vec8* kd = reinterpret_cast<vec8*>(Ks[b] + (wave * KS + 2 * f) * 1024) + lane;
-      kd[0] = widen<E>(kr[f].x, kr[f].y);
-      kd[64] = widen<E>(kr[f].z, kr[f].w);
-      f16x8_t* vd = reinterpret_cast<f16x8_t*>(Vs[b] + (HF * wave + f) * 2048) + lane;
-      vd[0] = widen_f16(vr[f].x, vr[f].y);
-      vd[64] = widen_f16(vr[f].z, vr[f].w);
-    }
-  };
-
-  if (tb < te) {
-    look_up(tb);
-    fetch(tb);
-    if (tb + 1 < te) look_up(tb + 1);
-    stage(tb, 0);
+  // Tiles [wb, we) are seen whole by every row, and all of their pages are there.
+  int wb = max(tb, (sees_lo(p, pos_base + last / p.group, len) + 63) >> 6);
+  int we = min(te, sees_hi(p, pos_base + row0 / p.group, len) >> 6);
+  if (wb < we) {
+    const int end = (we * 64 - 1) >> c.page_log2;
+    int gone = 0;
+    for (int e = ((wb * 64) >> c.page_log2) + tid; e <= end; e += 256) gone |= (unsigned)table[e] >= (unsigned)c.num_pages;
+    if (__syncthreads_or(gone)) wb = we = te;
+  } else {
+    wb = we = te;
   }
-  for (int tile = tb; tile < te; ++tile) {
-    const int b = (tile - tb) & 1;
-    const int ke = min(max(ke_n, kKvExpMin), kKvExpMax), ve = min(max(ve_n, kKvExpMin), kKvExpMax);
-    const bool here = here_n;
-    barrier_lds_reads_done();  // this tile is in LDS, and the other buffer is no longer read
-    if (tile + 1 < te) {
-      fetch(tile + 1);
-      if (tile + 2 < te) look_up(tile + 2);
+
+  // Pieces of a tile that this thread brings: of 16-key tile `wave` of K row m's 16 channels 64 f + 16 g .. of each
+  // f; of V channels 16 (HF wave + f) + m, keys 16 g .. + 15.  Their pages are looked up a tile ahead.
+  const int k_lane = ((UNI ? 16 * (m >> 2) : 0) + 4 * wave + (m & 3)) * DIM + 16 * g;
+  const int v_lane = ((16 * HF * wave + m) << c.page_log2) + (UNI ? 16 * g : 0);
+  auto k_key = [&](int tile) { return UNI ? tile * 64 : tile * 64 + 16 * (m >> 2); };
+  auto v_key = [&](int tile) { return UNI ? tile * 64 : tile * 64 + 16 * g; };
+  uint4 kr[HF], vr[HF];
+  int ke_n = 0, ve_n = 0;  // exponents of the lane's keys 16 g .. + 15
+  auto fetch_k = [&](int tile, int id) {
+    const uint8_t* at = c.k + ((((int64_t)id * c.heads + hk) << c.page_log2) + (k_key(tile) & (page - 1))) * DIM + k_lane;
+#pragma unroll
+    for (int f = 0; f < HF; ++f) kr[f] = *reinterpret_cast<const uint4*>(at + 64 * f);
+  };
+  auto fetch_v = [&](int tile, int id) {
+    const int64_t n = (int64_t)id * c.heads + hk;
+    const uint8_t* at = c.v + ((n * DIM) << c.page_log2) + (v_key(tile) & (page - 1)) + v_lane;
+#pragma unroll
+    for (int f = 0; f < HF; ++f) vr[f] = *reinterpret_cast<const uint4*>(at + ((16 * f) << c.page_log2));
+    ke_n = c.k_exp[n];
+    ve_n = c.v_exp[n];
+  };
+  auto stage_k = [&](int b) {
+#pragma unroll
+    for (int f = 0; f < HF; ++f) {
+      vec8* d = reinterpret_cast<vec8*>(Ks[b] + (wave * KS + 2 * f) * 1024) + lane;
+      d[0] = widen<E>(kr[f].x, kr[f].y);
+      d[64] = widen<E>(kr[f].z, kr[f].w);
     }
-    f32x4_t s[4][2];
+  };
+  auto stage_v = [&](int b) {
+#pragma unroll
+    for (int f = 0; f < HF; ++f) {
+      f16x8_t* d = reinterpret_cast<f16x8_t*>(Vs[b] + (HF * wave + f) * 2048) + lane;
+      d[0] = widen_f16(vr[f].x, vr[f].y);
+      d[64] = widen_f16(vr[f].z, vr[f].w);
+    }
+  };
+  auto scores = [&](int b, f32x4_t (&s)[4][2]) {
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -623,53 +624,234 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int64_t 
 #pragma unroll
         for (int q = 0; q < 2; ++q) s[t][q] = E::mfma16(a, qf[q][k], s[t][q]);
       }
-    const int j0 = tile * 64, jv = j0 + 16 * g;
-    const bool whole = j0 >= w_lo && j0 + 64 <= w_hi && __all(here);
-    if (!whole) {
+  };
+  auto pv = [&](int b, const f16x8_t (&pf)[2][2], auto fix) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+      for (int dt = 0; dt < DT; ++dt) {
+        const f16x8_t a = as_vec8<F16>(fix(*(reinterpret_cast<const uint4*>(Vs[b] + (2 * dt + u) * 1024) + lane)));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = jv + 4 * t + i;
-            if (!here || j < lo[q] || j >= hi[q]) s[t][q][i] = -INFINITY;
-          }
+        for (int q = 0; q < 2; ++q) o[dt][q] = F16::mfma16(a, pf[u][q], o[dt][q]);
+      }
+  };
+
+  // Tiles that some row sees in part, or whose pages are not all there: one at a time.
+  auto part_tiles = [&](int t0, int t1) {
+    if (t0 >= t1) return;
+    int lo[2], hi[2];  // what the lane's rows see
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      int tok, head;
+      row_of(q, tok, head);
+      lo[q] = sees_lo(p, pos_base + tok, len);
+      hi[q] = sees_hi(p, pos_base + tok, len);
     }
-    const float sc = ldexpf(p.scale, ke);
-    f16x8_t pf[2][2];
+    for (int tile = t0; tile < t1; ++tile) {
+      auto page_of = [&](int j) -> int {
+        const int id = j < len ? table[j >> c.page_log2] : -1;
+        return (unsigned)id < (unsigned)c.num_pages ? id : -1;
+      };
+      const int vid = page_of(v_key(tile));
+      const bool here = vid >= 0;
+      const int jv = tile * 64 + 16 * g;
+      fetch_k(tile, max(page_of(k_key(tile)), 0));
+      fetch_v(tile, max(vid, 0));
+      const int nb = here ? min(max(len - jv, 0), 16) : 0;  // codes behind the last key are whatever the page held
 #pragma unroll
-    for (int q = 0; q < 2; ++q) softmax_step<DT, 2>(s, q, sc, ve, m_run[q], l_run[q], o, pf[0][q], pf[1][q]);
-    auto pv = [&](auto fix) {
+      for (int f = 0; f < HF; ++f)
+        vr[f] = make_uint4(vr[f].x & first_bytes(nb), vr[f].y & first_bytes(nb - 4), vr[f].z & first_bytes(nb - 8), vr[f].w & first_bytes(nb - 12));
+      barrier_lds_reads_done();
+      stage_k(0);
+      stage_v(0);
+      barrier_lds_reads_done();
+      f32x4_t s[4][2];
+      scores(0, s);
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int q = 0; q < 2; ++q) {
+        // Key jv + e is hidden for e below a and from b on.
+        const int a = here ? lo[q] - jv : 16, b = here ? hi[q] - jv : 0;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const f16x8_t a = as_vec8<F16>(fix(*(reinterpret_cast<const uint4*>(Vs[b] + (2 * dt + u) * 1024) + lane)));
-#pragma unroll
-          for (int q = 0; q < 2; ++q) o[dt][q] = F16::mfma16(a, pf[u][q], o[dt][q]);
+        for (int e = 0; e < 16; ++e) {
+          const float x = s[e >> 2][q][e & 3];
+          s[e >> 2][q][e & 3] = ((e >= a) & (e < b)) ? x : -INFINITY;
         }
-    };
-    if (whole) {
-      pv([](const uint4& w) { return w; });
-    } else {
-      poison_step<DT>(Vs[b], lane, here, jv, lo, hi, o);
-      pv([](const uint4& w) { return make_uint4(finite_halves(w.x), finite_halves(w.y), finite_halves(w.z), finite_halves(w.w)); });
+      }
+      const int ke = page_exp(ke_n), ve = page_exp(ve_n);
+      const float sc = p.scale * exp2_int(ke), vf = (float)ve, inv = exp2_int(-ve);
+      f16x8_t pf[2][2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        raise_max<DT, 2>(lane_max<2>(s, q, sc, vf), q, m_run[q], l_run[q], o);
+        weights<2>(s, q, sc, vf, inv, m_run[q], l_run[q], pf[0][q], pf[1][q]);
+      }
+      poison_step<DT>(Vs[0], lane, here, jv, lo, hi, o);
+      pv(0, pf, [](const uint4& w) { return make_uint4(finite_halves(w.x), finite_halves(w.y), finite_halves(w.z), finite_halves(w.w)); });
     }
-    if (tile + 1 < te) stage(tile + 1, b ^ 1);
+  };
+
+  part_tiles(tb, wb);
+  if (wb < we) {
+    // Scores run a tile ahead of the weights and sums: at the top of a step K of tile + 1 and V of tile are in LDS and s
+    // holds the tile's scores.  The scores of the next tile and the weights of this one need nothing of each other, nor
+    // do the sums and the widening of what comes next: matrix and vector instructions run in each other's time.
+    // Page of the lane's key j, or with UNI of the tile's: from a vector register that holds the next 64 table entries
+    // (scalar loads would make every wait for an LDS read a wait for all of them).
+    int held = 0, held_at = -64;
+    auto look = [&](int j) -> int {
+      const int e = j >> c.page_log2;
+      if constexpr (UNI) {
+        if (e >= held_at + 64) {
+          held_at = e;
+          held = table[min(e + lane, (we * 64 - 1) >> c.page_log2)];
+        }
+        return __builtin_amdgcn_readlane(held, e - held_at);
+      } else {
+        return table[e];
+      }
+    };
+    auto clip = [&](int tile) { return min(tile, we - 1); };
+    auto as_is = [](const uint4& w) { return w; };
+    f32x4_t sa[4][2], sb[4][2];
+    float sc, vf, inv, mx[2];
+    auto scales = [&] {
+      const int ke = page_exp(UNI ? __builtin_amdgcn_readfirstlane(ke_n) : ke_n);
+      const int ve = page_exp(UNI ? __builtin_amdgcn_readfirstlane(ve_n) : ve_n);
+      sc = p.scale * exp2_int(ke);
+      vf = (float)ve;
+      inv = exp2_int(-ve);
+    };
+    fetch_k(wb, look(k_key(wb)));
+    fetch_v(wb, look(v_key(wb)));
+    barrier_lds_reads_done();
+    stage_k(0);
+    stage_v(0);
+    scales();
+    fetch_k(clip(wb + 1), look(k_key(clip(wb + 1))));
+    int vid = look(v_key(clip(wb + 1))), kid = look(k_key(clip(wb + 2)));
+    barrier_lds_reads_done();
+    scores(0, sa);
+    stage_k(1);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) mx[q] = lane_max<2>(sa, q, sc, vf);
+    barrier_lds_reads_done();
+    auto step = [&](int tile, int b, f32x4_t (&s)[4][2], f32x4_t (&sn)[4][2]) {
+      fetch_k(clip(tile + 2), kid);
+      fetch_v(tile + 1, vid);
+      vid = UNI ? kid : look(v_key(clip(tile + 2)));
+      kid = look(k_key(clip(tile + 3)));
+#pragma unroll
+      for (int q = 0; q < 2; ++q) raise_max<DT, 2>(mx[q], q, m_run[q], l_run[q], o);
+      // One operand at a time, read kAhead operands before, and its two MFMAs; between them, first the weights of 32 / NF
+      // scores, then a piece of the next tiles' codes widened and a share of the maxima.  The order is fixed
+      // (sched_barrier): left alone, the compiler reads each operand where it is used and runs the two kinds apart.
+      constexpr int NF = KS * 4, PAIRS = 16 / NF;  // operands of K, and of V
+      static_assert(NF == 2 * DT && 8 * HF == NF, "two operands for each channel tile of V and each piece to widen");
+      uint4 fr[2 * NF];
+      auto read = [&](int f) {
+        if (f >= 2 * NF) return;
+        const int v = f - NF;
+        fr[f] = f < NF ? *(reinterpret_cast<const uint4*>(Ks[b ^ 1] + ((f % 4) * KS + f / 4) * 1024) + lane)
+                       : *(reinterpret_cast<const uint4*>(Vs[b] + (2 * (v % DT) + v / DT) * 1024) + lane);
+      };
+#pragma unroll
+      for (int f = 0; f < kAhead; ++f) read(f);
+      float off[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < 2; ++q) off[q] = vf - m_run[q] + kShift;
+      uint32_t w[2][8];
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        read(f + kAhead);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          sn[f % 4][q] = E::mfma16(as_vec8<E>(fr[f]), qf[q][f / 4], f < 4 ? (f32x4_t){0.f, 0.f, 0.f, 0.f} : sn[f % 4][q]);
+#pragma unroll
+        for (int n = f * PAIRS; n < (f + 1) * PAIRS; ++n) {
+          const int q = n & 1, e = n >> 1;
+          const f32x4_t& x = s[e >> 1][q];
+          const float p0 = fast_exp2(fmaf(x[2 * (e & 1)], sc, off[q]));
+          const float p1 = fast_exp2(fmaf(x[2 * (e & 1) + 1], sc, off[q]));
+          w[q][e] = F16::pack2(p0, p1);
+          sum[q] += p0 + p1;
+          asm volatile("" : "+v"(sum[q]));  // added here: sunk behind the loop, the sums would keep 32 weights in registers
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      f16x8_t pf[2][2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        l_run[q] = fmaf(sum[q], inv, l_run[q]);
+        pf[0][q] = as_vec8<F16>((u32x4_t){w[q][0], w[q][1], w[q][2], w[q][3]});
+        pf[1][q] = as_vec8<F16>((u32x4_t){w[q][4], w[q][5], w[q][6], w[q][7]});
+        mx[q] = -INFINITY;
+      }
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        read(NF + f + kAhead);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) o[f % DT][q] = F16::mfma16(as_vec8<F16>(fr[NF + f]), pf[f / DT][q], o[f % DT][q]);
+        // Pieces: the two halves of each kr, then of each vr.
+        const int i = f / 2;
+        if (f % 2 && i < NF / 4) {
+          vec8* d = reinterpret_cast<vec8*>(Ks[b] + (wave * KS + i) * 1024) + lane;
+          d[0] = i % 2 ? widen<E>(kr[i / 2].z, kr[i / 2].w) : widen<E>(kr[i / 2].x, kr[i / 2].y);
+        } else if (f % 2) {
+          const int n = (i - NF / 4) / 2;
+          f16x8_t* d = reinterpret_cast<f16x8_t*>(Vs[b ^ 1] + (HF * wave + n) * 2048 + (i % 2) * 1024) + lane;
+          d[0] = i % 2 ? widen_f16(vr[n].z, vr[n].w) : widen_f16(vr[n].x, vr[n].y);
+        }
+#pragma unroll
+        for (int n = f * PAIRS; n < (f + 1) * PAIRS; ++n) {
+          const int q = n & 1, e = n >> 1;
+          const f32x4_t& x = sn[e >> 1][q];
+          mx[q] = fmaxf(fmaxf(x[2 * (e & 1)], x[2 * (e & 1) + 1]), mx[q]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      scales();
+#pragma unroll
+      for (int q = 0; q < 2; ++q) mx[q] = fmaf(mx[q], sc, vf);
+      barrier_lds_reads_done();
+    };
+    auto finish = [&](int b, const f32x4_t (&s)[4][2]) {
+      f16x8_t pf[2][2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        raise_max<DT, 2>(mx[q], q, m_run[q], l_run[q], o);
+        weights<2>(s, q, sc, vf, inv, m_run[q], l_run[q], pf[0][q], pf[1][q]);
+      }
+      pv(b, pf, as_is);
+    };
+    int tile = wb;
+    for (; tile + 2 < we; tile += 2) {
+      step(tile, 0, sa, sb);
+      step(tile + 1, 1, sb, sa);
+    }
+    if (tile + 1 < we) {
+      step(tile, 0, sa, sb);
+      finish(1, sb);
+    } else {
+      finish(0, sa);
+    }
   }
+  part_tiles(we, te);
 
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const float l = quad16_sum(l_run[q]);
     if (wrow + 16 * q + m >= rows) continue;
+    int tok, head;
+    row_of(q, tok, head);
+    const int64_t at_tok = tok0 + tok;
     if (p.splits == 1) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float w = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) store4(p, qtok[q], qhead[q], 16 * dt + 4 * g, o[dt][q], inv);
-      if (g == 0 && p.lse) p.lse[qtok[q] * p.q_heads + qhead[q]] = row_lse(m_run[q], l);
+      for (int dt = 0; dt < DT; ++dt) store4(p, at_tok, head, 16 * dt + 4 * g, o[dt][q], w);
+      if (g == 0 && p.lse) p.lse[at_tok * p.q_heads + head] = row_lse(m_run[q], l);
     } else {
-      const int64_t at = (int64_t)z * p.tokens * p.q_heads + qtok[q] * p.q_heads + qhead[q];
+      const int64_t at = ((int64_t)z * p.tokens + at_tok) * p.q_heads + head;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(p.part_o + at * DIM + 16 * dt + 4 * g) = o[dt][q];
       if (g == 0) {
@@ -727,7 +909,11 @@ hipError_t launch_tiles(const KvAttnParams& p, hipStream_t stream) {
   const int64_t items = tiles * p.c.heads * p.splits;
   const int64_t per_xcd = (items + 7) / 8;
   if (per_xcd * 8 > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((kv_attn_tiles<E, DIM>), dim3((unsigned)(per_xcd * 8)), dim3(256), 0, stream, p, tiles, items, per_xcd);
+  const dim3 grid((unsigned)(per_xcd * 8));
+  if (p.c.page_log2 >= 6)
+    hipLaunchKernelGGL((kv_attn_tiles<E, DIM, true>), grid, dim3(256), 0, stream, p, (int)tiles, (int)items, (int)per_xcd);
+  else
+    hipLaunchKernelGGL((kv_attn_tiles<E, DIM, false>), grid, dim3(256), 0, stream, p, (int)tiles, (int)items, (int)per_xcd);
   return hipGetLastError();
 }
 
@@ -743,25 +929,35 @@ hipError_t launch_any(const KvAttnParams& p, int rows, hipStream_t stream) {
 
 }  // namespace
 
-// Tile and parts of the keys, from the sizes that the host knows.
-KvAttnPlan kv_attn_plan(int64_t tokens, int requests, int q_heads, int kv_heads, int64_t max_kv) {
+// Tile and parts of the keys, from the sizes that the host knows.  A tile of 16 rows is bound by the bytes of the keys,
+// one of 128 by the matrix units; both run in rounds of as many workgroups as the chip holds at once, and a part of the
+// keys more makes the last round shorter but its sums pass through memory.  The parts with the least time are taken.
+KvAttnPlan kv_attn_plan(int64_t tokens, int requests, int q_heads, int kv_heads, int dim, int64_t max_kv) {
   const int group = q_heads / kv_heads;
   const int64_t mean = (tokens * group + requests - 1) / requests;
   KvAttnPlan plan;
   plan.rows = mean <= 16 ? 16 : 128;
-  const int64_t wgs = ((tokens * group + plan.rows - 1) / plan.rows + (mean % plan.rows ? requests - 1 : 0)) * kv_heads;
-  // Four tiles a part at least; enough parts for two workgroups on each compute unit.
-  const int64_t most = (max_kv + 255) / 256;
-  int64_t want = ((plan.rows == 16 ? 1024 : 512) + wgs - 1) / wgs;
-  if (want > most) want = most;
-  if (want > 64) want = 64;
-  if (want < 1) want = 1;
-  plan.splits = (int)want;
+  const double wgs = (double)((mean + plan.rows - 1) / plan.rows) * requests * kv_heads;
+  const double slots = plan.rows == 16 ? 768 : 512;
+  const double work_us = plan.rows == 16 ? 2.0 * requests * max_kv * kv_heads * dim / 5.5e6
+                                         : 4.0 * tokens * max_kv * q_heads * dim / 1e9;
+  const double part_us = 2.0 * tokens * q_heads * (dim + 2) * sizeof(float) / 4.5e6;  // written and read
+  const int64_t most = (max_kv + 255) / 256 < 64 ? (max_kv + 255) / 256 : 64;        // four tiles a part at least
+  plan.splits = 1;
+  double best = 0.0;
+  for (int n = 1; n <= most; ++n) {
+    const double used = wgs * n, rounds = ceil(used / slots);
+    const double t = work_us * rounds * slots / used + (n > 1 ? 4.0 + n * part_us : 0.0);
+    if (n == 1 || t < best) {
+      best = t;
+      plan.splits = n;
+    }
+  }
   return plan;
 }
 
 hipError_t launch_kv_attn(const KvAttnParams& p, hipStream_t stream) {
-  const KvAttnPlan plan = kv_attn_plan(p.tokens, p.requests, p.q_heads, p.c.heads, p.max_kv);
+  const KvAttnPlan plan = kv_attn_plan(p.tokens, p.requests, p.q_heads, p.c.heads, p.c.dim, p.max_kv);
   if (plan.splits != p.splits) return hipErrorInvalidValue;
   if (p.c.dim == 128) return p.f16 ? launch_any<F16, 128>(p, plan.rows, stream) : launch_any<Bf16, 128>(p, plan.rows, stream);
   if (p.c.dim == 64) return p.f16 ? launch_any<F16, 64>(p, plan.rows, stream) : launch_any<Bf16, 64>(p, plan.rows, stream);

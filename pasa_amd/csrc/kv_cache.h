@@ -107,6 +107,7 @@ struct KvAttnParams {
   const int32_t* cu_q;  // nullptr: tokens / requests for each request
   int requests;
   int64_t tokens;
+  int per_request;  // tokens / requests
   int q_heads;
   int group;        // q_heads / heads
   int64_t max_kv;   // keys from here on are not looked at
@@ -124,7 +125,7 @@ struct KvAttnPlan {
   int rows;    // rows of a workgroup's tile
   int splits;
 };
-KvAttnPlan kv_attn_plan(int64_t tokens, int requests, int q_heads, int kv_heads, int64_t max_kv);
+KvAttnPlan kv_attn_plan(int64_t tokens, int requests, int q_heads, int kv_heads, int dim, int64_t max_kv);
 hipError_t launch_kv_attn(const KvAttnParams& p, hipStream_t stream);
 
 }  // namespace pasa
