@@ -116,7 +116,7 @@ __device__ __forceinline__ float row_lse(float top, float l) {
 template <int TILE, int DIM>
 __device__ __forceinline__ void zero_rows(const KvAttnParams& p, int hk, int z, int tok0, int rows, int row0) {
   if (!p.zero_tail || z != 0 || p.splits != 1) return;  // with parts, the join writes them
-  for (int e = threadIdx.x; e < TILE * DIM; e += 256) {
+  for (int e = threadIdx.x; e < TILE * DIM; e += blockDim.x) {
     const int i = row0 + e / DIM;
     if (i >= rows) break;
     const int64_t tok = tok0 + i / p.group;
@@ -168,19 +168,29 @@ __device__ __forceinline__ float lane_max(const f32x4_t (&s)[4][NQ], int q, floa
   return fmaf(mx, sc, ve);
 }
 
-// The running maximum of row tile q, and o and l scaled where it rose.  A rise by less than kSlack is left alone: p then
-// stays below 2^(kShift + kSlack), inside fp16, and scaling o's registers is rare.
+// The running maxima, and o and l scaled where one rose.  A rise by less than kSlack is left alone: p then stays below
+// 2^(kShift + kSlack), inside fp16, and scaling o's registers is rare.
 template <int DT, int NQ>
-__device__ __forceinline__ void raise_max(float mx, int q, float& m_run, float& l_run, f32x4_t (&o)[DT][NQ]) {
-  if (__any(mx > m_run + kSlack)) {
-    const float m_new = fmaxf(m_run, quad16_max(mx));
-    const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
-    m_run = m_new;
-    l_run *= alpha;
+__device__ __forceinline__ void raise_max(const float (&mx)[NQ], float (&m_run)[NQ], float (&l_run)[NQ], f32x4_t (&o)[DT][NQ]) {
+  bool rise = false;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) rise = rise | (mx[q] > m_run[q] + kSlack);
+  if (__builtin_expect(!__any(rise), 1)) return;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const float m_new = fmaxf(m_run[q], quad16_max(mx[q]));
+    const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run[q] - m_new);
+    m_run[q] = m_new;
+    l_run[q] *= alpha;
+    // In place (a plain product makes the compiler copy all of o on the path around it).
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[dt][q][i] *= alpha;
+      for (int i = 0; i < 4; ++i) {
+        float x = o[dt][q][i];
+        asm("v_mul_f32 %0, %1, %0" : "+v"(x) : "v"(alpha));
+        o[dt][q][i] = x;
+      }
   }
 }
 
@@ -394,9 +404,12 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
     }
     const float sc = p.scale * exp2_int(ke), inv = exp2_int(-ve);
     f16x8_t pf[2][NQ];
+    float mx[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) mx[q] = lane_max<NQ>(s, q, sc, (float)ve);
+    raise_max<DT, NQ>(mx, m_run, l_run, o);
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
-      raise_max<DT, NQ>(lane_max<NQ>(s, q, sc, (float)ve), q, m_run[q], l_run[q], o);
       weights<NQ>(s, q, sc, (float)ve, inv, m_run[q], l_run[q], pf[0][q], pf[1][q]);
     }
     if (poison) {
@@ -494,20 +507,24 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
 // waves' MFMAs read (1 KB pieces, lane after lane: no bank conflicts either way), while the tile before is computed.
 // Two buffers, one barrier a tile.  Widening once for 128 rows costs 32 conversions a thread and tile of 16-bit LDS
 // traffic; widening after the LDS read would cost each wave 128.
-template <int DIM>
+template <int DIM, int WAVES>
 struct KvTile {
-  static constexpr int ROWS = 128;
+  static constexpr int ROWS = 32 * WAVES;
   static constexpr int KS = DIM / 32, DT = DIM / 16, HF = DIM / 64;
+  static constexpr int NP = 4 * HF / WAVES;  // 1 KB pieces of K, and of V, that a wave brings of a tile
   static constexpr int KBYTES = 64 * DIM * 2, VBYTES = KBYTES;
+  static_assert(NP >= 1, "every wave brings a piece");
 };
 
 constexpr int kAhead = 4;  // LDS reads in flight
 
 // UNI: pages of 64 tokens and more, so that a tile has one page and its number stays in scalar registers.
-template <typename E, int DIM, bool UNI>
-__global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int tiles, int items, int per_xcd) {
-  using C = KvTile<DIM>;
-  constexpr int KS = C::KS, DT = C::DT, HF = C::HF;
+template <typename E, int DIM, int WAVES, bool UNI>
+__global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, int tiles, int items, int per_xcd) {
+  using C = KvTile<DIM, WAVES>;
+  constexpr int KS = C::KS, DT = C::DT, NP = C::NP;
+  // Tiles are fetched a step before they are widened; with eight waves two steps, for a wave then holds half as much.
+  constexpr int SETS = WAVES == 8 ? 2 : 1;
   using vec8 = typename E::vec8;
   __shared__ __attribute__((aligned(1024))) unsigned char Ks[2][C::KBYTES];
   __shared__ __attribute__((aligned(1024))) unsigned char Vs[2][C::VBYTES];
@@ -568,48 +585,48 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int tile
   if (wb < we) {
     const int end = (we * 64 - 1) >> c.page_log2;
     int gone = 0;
-    for (int e = ((wb * 64) >> c.page_log2) + tid; e <= end; e += 256) gone |= (unsigned)table[e] >= (unsigned)c.num_pages;
+    for (int e = ((wb * 64) >> c.page_log2) + tid; e <= end; e += 64 * WAVES) gone |= (unsigned)table[e] >= (unsigned)c.num_pages;
     if (__syncthreads_or(gone)) wb = we = te;
   } else {
     wb = we = te;
   }
 
-  // Pieces of a tile that this thread brings: of 16-key tile `wave` of K row m's 16 channels 64 f + 16 g .. of each
-  // f; of V channels 16 (HF wave + f) + m, keys 16 g .. + 15.  Their pages are looked up a tile ahead.
-  const int k_lane = ((UNI ? 16 * (m >> 2) : 0) + 4 * wave + (m & 3)) * DIM + 16 * g;
-  const int v_lane = ((16 * HF * wave + m) << c.page_log2) + (UNI ? 16 * g : 0);
+  // Pieces of a tile that this thread brings: of 16-key tile kt of K row m's 16 channels 64 f + 16 g .. of NP halves f
+  // from kf on; of V channels 16 (NP wave + n) + m, keys 16 g .. + 15.  Their pages are looked up a step ahead.
+  const int kt = wave & 3, kf = WAVES == 8 ? wave >> 2 : 0;
+  const int k_lane = ((UNI ? 16 * (m >> 2) : 0) + 4 * kt + (m & 3)) * DIM + 64 * kf + 16 * g;
+  const int v_lane = ((16 * NP * wave + m) << c.page_log2) + (UNI ? 16 * g : 0);
   auto k_key = [&](int tile) { return UNI ? tile * 64 : tile * 64 + 16 * (m >> 2); };
   auto v_key = [&](int tile) { return UNI ? tile * 64 : tile * 64 + 16 * g; };
-  uint4 kr[HF], vr[HF];
-  int ke_n = 0, ve_n = 0;  // exponents of the lane's keys 16 g .. + 15
-  auto fetch_k = [&](int tile, int id) {
+  uint4 kr[SETS][NP], vr[SETS][NP];
+  int ke_n[SETS], ve_n[SETS];  // exponents of the lane's keys 16 g .. + 15
+  auto fetch_k = [&](int set, int tile, int id) {
     const uint8_t* at = c.k + ((((int64_t)id * c.heads + hk) << c.page_log2) + (k_key(tile) & (page - 1))) * DIM + k_lane;
 #pragma unroll
-    for (int f = 0; f < HF; ++f) kr[f] = *reinterpret_cast<const uint4*>(at + 64 * f);
+    for (int n = 0; n < NP; ++n) kr[set][n] = *reinterpret_cast<const uint4*>(at + 64 * n);
   };
-  auto fetch_v = [&](int tile, int id) {
-    const int64_t n = (int64_t)id * c.heads + hk;
-    const uint8_t* at = c.v + ((n * DIM) << c.page_log2) + (v_key(tile) & (page - 1)) + v_lane;
+  auto fetch_v = [&](int set, int tile, int id) {
+    const int64_t row = (int64_t)id * c.heads + hk;
+    const uint8_t* at = c.v + ((row * DIM) << c.page_log2) + (v_key(tile) & (page - 1)) + v_lane;
 #pragma unroll
-    for (int f = 0; f < HF; ++f) vr[f] = *reinterpret_cast<const uint4*>(at + ((16 * f) << c.page_log2));
-    ke_n = c.k_exp[n];
-    ve_n = c.v_exp[n];
+    for (int n = 0; n < NP; ++n) vr[set][n] = *reinterpret_cast<const uint4*>(at + ((16 * n) << c.page_log2));
+    ke_n[set] = c.k_exp[row];
+    ve_n[set] = c.v_exp[row];
   };
-  auto stage_k = [&](int b) {
-#pragma unroll
-    for (int f = 0; f < HF; ++f) {
-      vec8* d = reinterpret_cast<vec8*>(Ks[b] + (wave * KS + 2 * f) * 1024) + lane;
-      d[0] = widen<E>(kr[f].x, kr[f].y);
-      d[64] = widen<E>(kr[f].z, kr[f].w);
-    }
+  // Half u of piece n, widened, into buffer b.
+  auto stage_k = [&](int b, int n, int u, const uint4& x) {
+    vec8* d = reinterpret_cast<vec8*>(Ks[b] + (kt * KS + 2 * (kf + n) + u) * 1024) + lane;
+    d[0] = u ? widen<E>(x.z, x.w) : widen<E>(x.x, x.y);
   };
-  auto stage_v = [&](int b) {
+  auto stage_v = [&](int b, int n, int u, const uint4& x) {
+    f16x8_t* d = reinterpret_cast<f16x8_t*>(Vs[b] + (NP * wave + n) * 2048 + u * 1024) + lane;
+    d[0] = u ? widen_f16(x.z, x.w) : widen_f16(x.x, x.y);
+  };
+  auto stage_all = [&](int b, const uint4 (&x)[NP], auto stage) {
 #pragma unroll
-    for (int f = 0; f < HF; ++f) {
-      f16x8_t* d = reinterpret_cast<f16x8_t*>(Vs[b] + (HF * wave + f) * 2048) + lane;
-      d[0] = widen_f16(vr[f].x, vr[f].y);
-      d[64] = widen_f16(vr[f].z, vr[f].w);
-    }
+    for (int n = 0; n < NP; ++n)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) stage(b, n, u, x[n]);
   };
   auto scores = [&](int b, f32x4_t (&s)[4][2]) {
 #pragma unroll
@@ -655,16 +672,19 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int tile
       const int vid = page_of(v_key(tile));
       const bool here = vid >= 0;
       const int jv = tile * 64 + 16 * g;
-      fetch_k(tile, max(page_of(k_key(tile)), 0));
-      fetch_v(tile, max(vid, 0));
+      fetch_k(0, tile, max(page_of(k_key(tile)), 0));
+      fetch_v(0, tile, max(vid, 0));
       const int nb = here ? min(max(len - jv, 0), 16) : 0;  // codes behind the last key are whatever the page held
 #pragma unroll
-      for (int f = 0; f < HF; ++f)
-        vr[f] = make_uint4(vr[f].x & first_bytes(nb), vr[f].y & first_bytes(nb - 4), vr[f].z & first_bytes(nb - 8), vr[f].w & first_bytes(nb - 12));
+      for (int n = 0; n < NP; ++n) {
+        uint4& x = vr[0][n];
+        x = make_uint4(x.x & first_bytes(nb), x.y & first_bytes(nb - 4), x.z & first_bytes(nb - 8), x.w & first_bytes(nb - 12));
+      }
       barrier_lds_reads_done();
-      stage_k(0);
-      stage_v(0);
+      stage_all(0, kr[0], stage_k);
+      stage_all(0, vr[0], stage_v);
       barrier_lds_reads_done();
+      if (wrow >= rows) continue;  // (of the whole wave) nothing to compute, but the other waves' tiles to bring
       f32x4_t s[4][2];
       scores(0, s);
 #pragma unroll
@@ -677,12 +697,15 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int tile
           s[e >> 2][q][e & 3] = ((e >= a) & (e < b)) ? x : -INFINITY;
         }
       }
-      const int ke = page_exp(ke_n), ve = page_exp(ve_n);
+      const int ke = page_exp(ke_n[0]), ve = page_exp(ve_n[0]);
       const float sc = p.scale * exp2_int(ke), vf = (float)ve, inv = exp2_int(-ve);
       f16x8_t pf[2][2];
+      float mx[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) mx[q] = lane_max<2>(s, q, sc, vf);
+      raise_max<DT, 2>(mx, m_run, l_run, o);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        raise_max<DT, 2>(lane_max<2>(s, q, sc, vf), q, m_run[q], l_run[q], o);
         weights<2>(s, q, sc, vf, inv, m_run[q], l_run[q], pf[0][q], pf[1][q]);
       }
       poison_step<DT>(Vs[0], lane, here, jv, lo, hi, o);
@@ -704,6 +727,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int tile
         if (e >= held_at + 64) {
           held_at = e;
           held = table[min(e + lane, (we * 64 - 1) >> c.page_log2)];
+          asm volatile("" : "+v"(held));  // waited for here, not at every use below, which would wait for the tiles' loads
         }
         return __builtin_amdgcn_readlane(held, e - held_at);
       } else {
@@ -714,39 +738,51 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int tile
     auto as_is = [](const uint4& w) { return w; };
     f32x4_t sa[4][2], sb[4][2];
     float sc, vf, inv, mx[2];
-    auto scales = [&] {
-      const int ke = page_exp(UNI ? __builtin_amdgcn_readfirstlane(ke_n) : ke_n);
-      const int ve = page_exp(UNI ? __builtin_amdgcn_readfirstlane(ve_n) : ve_n);
+    auto scales = [&](int set) {
+      const int ke = page_exp(UNI ? __builtin_amdgcn_readfirstlane(ke_n[set]) : ke_n[set]);
+      const int ve = page_exp(UNI ? __builtin_amdgcn_readfirstlane(ve_n[set]) : ve_n[set]);
       sc = p.scale * exp2_int(ke);
       vf = (float)ve;
       inv = exp2_int(-ve);
     };
-    fetch_k(wb, look(k_key(wb)));
-    fetch_v(wb, look(v_key(wb)));
+    // Step `tile` widens K of tile + 2 and V of tile + 1 from its set, and fetches those SETS - 1 tiles on into the other.
+    constexpr int KN = SETS + 1;  // K's distance when it is fetched (V's: SETS)
+    int vid, kid;
+    auto look_next = [&](int tile) {  // pages of what step `tile` fetches
+      vid = look(v_key(clip(tile + SETS)));
+      kid = look(k_key(clip(tile + KN)));
+    };
+    fetch_k(0, wb, look(k_key(wb)));
+    fetch_v(0, wb, look(v_key(wb)));
     barrier_lds_reads_done();
-    stage_k(0);
-    stage_v(0);
-    scales();
-    fetch_k(clip(wb + 1), look(k_key(clip(wb + 1))));
-    int vid = look(v_key(clip(wb + 1))), kid = look(k_key(clip(wb + 2)));
+    stage_all(0, kr[0], stage_k);
+    stage_all(0, vr[0], stage_v);
+    scales(0);
+    int id1v = look(v_key(clip(wb + 1)));
+    fetch_k(0, clip(wb + 1), look(k_key(clip(wb + 1))));
+    if constexpr (SETS == 2) {
+      fetch_v(1, clip(wb + 1), id1v);
+      fetch_k(1, clip(wb + 2), look(k_key(clip(wb + 2))));
+    }
+    look_next(wb);
+    if constexpr (SETS == 1) vid = id1v;
     barrier_lds_reads_done();
     scores(0, sa);
-    stage_k(1);
+    stage_all(1, kr[0], stage_k);
 #pragma unroll
     for (int q = 0; q < 2; ++q) mx[q] = lane_max<2>(sa, q, sc, vf);
     barrier_lds_reads_done();
     auto step = [&](int tile, int b, f32x4_t (&s)[4][2], f32x4_t (&sn)[4][2]) {
-      fetch_k(clip(tile + 2), kid);
-      fetch_v(tile + 1, vid);
-      vid = UNI ? kid : look(v_key(clip(tile + 2)));
-      kid = look(k_key(clip(tile + 3)));
-#pragma unroll
-      for (int q = 0; q < 2; ++q) raise_max<DT, 2>(mx[q], q, m_run[q], l_run[q], o);
+      const int fs = SETS == 2 ? b : 0, ss = SETS == 2 ? b ^ 1 : 0;  // sets to fetch into, to widen from
+      fetch_k(fs, clip(tile + KN), kid);
+      fetch_v(fs, clip(tile + SETS), vid);
+      look_next(tile + 1);
+      raise_max<DT, 2>(mx, m_run, l_run, o);
       // One operand at a time, read kAhead operands before, and its two MFMAs; between them, first the weights of 32 / NF
       // scores, then a piece of the next tiles' codes widened and a share of the maxima.  The order is fixed
       // (sched_barrier): left alone, the compiler reads each operand where it is used and runs the two kinds apart.
       constexpr int NF = KS * 4, PAIRS = 16 / NF;  // operands of K, and of V
-      static_assert(NF == 2 * DT && 8 * HF == NF, "two operands for each channel tile of V and each piece to widen");
+      static_assert(NF == 2 * DT && NF % (4 * NP) == 0, "two operands for each channel tile of V and each piece to widen");
       uint4 fr[2 * NF];
       auto read = [&](int f) {
         if (f >= 2 * NF) return;
@@ -792,34 +828,31 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles(KvAttnParams p, int tile
         read(NF + f + kAhead);
 #pragma unroll
         for (int q = 0; q < 2; ++q) o[f % DT][q] = F16::mfma16(as_vec8<F16>(fr[NF + f]), pf[f / DT][q], o[f % DT][q]);
-        // Pieces: the two halves of each kr, then of each vr.
-        const int i = f / 2;
-        if (f % 2 && i < NF / 4) {
-          vec8* d = reinterpret_cast<vec8*>(Ks[b] + (wave * KS + i) * 1024) + lane;
-          d[0] = i % 2 ? widen<E>(kr[i / 2].z, kr[i / 2].w) : widen<E>(kr[i / 2].x, kr[i / 2].y);
-        } else if (f % 2) {
-          const int n = (i - NF / 4) / 2;
-          f16x8_t* d = reinterpret_cast<f16x8_t*>(Vs[b ^ 1] + (HF * wave + n) * 2048 + (i % 2) * 1024) + lane;
-          d[0] = i % 2 ? widen_f16(vr[n].z, vr[n].w) : widen_f16(vr[n].x, vr[n].y);
+        constexpr int EVERY = NF / (4 * NP);  // one half of a piece of K, then of V, every so many operands
+        if (f % EVERY == EVERY - 1) {
+          const int i = f / EVERY;
+          if (i < 2 * NP) stage_k(b, i / 2, i % 2, kr[ss][i / 2]);
+          else stage_v(b ^ 1, i / 2 - NP, i % 2, vr[ss][i / 2 - NP]);
         }
 #pragma unroll
         for (int n = f * PAIRS; n < (f + 1) * PAIRS; ++n) {
           const int q = n & 1, e = n >> 1;
           const f32x4_t& x = sn[e >> 1][q];
           mx[q] = fmaxf(fmaxf(x[2 * (e & 1)], x[2 * (e & 1) + 1]), mx[q]);
+          asm volatile("" : "+v"(mx[q]));
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      scales();
+      scales(ss);
 #pragma unroll
       for (int q = 0; q < 2; ++q) mx[q] = fmaf(mx[q], sc, vf);
       barrier_lds_reads_done();
     };
     auto finish = [&](int b, const f32x4_t (&s)[4][2]) {
       f16x8_t pf[2][2];
+      raise_max<DT, 2>(mx, m_run, l_run, o);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        raise_max<DT, 2>(mx[q], q, m_run[q], l_run[q], o);
         weights<2>(s, q, sc, vf, inv, m_run[q], l_run[q], pf[0][q], pf[1][q]);
       }
       pv(b, pf, as_is);
@@ -903,23 +936,26 @@ hipError_t launch_rows(const KvAttnParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename E, int DIM>
+template <typename E, int DIM, int WAVES>
 hipError_t launch_tiles(const KvAttnParams& p, hipStream_t stream) {
-  const int64_t tiles = p.tokens * p.group / KvTile<DIM>::ROWS + p.requests + 1;
+  const int64_t tiles = p.tokens * p.group / KvTile<DIM, WAVES>::ROWS + p.requests + 1;
   const int64_t items = tiles * p.c.heads * p.splits;
   const int64_t per_xcd = (items + 7) / 8;
   if (per_xcd * 8 > 0x7fffffff) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)(per_xcd * 8));
+  const dim3 grid((unsigned)(per_xcd * 8)), block(64 * WAVES);
   if (p.c.page_log2 >= 6)
-    hipLaunchKernelGGL((kv_attn_tiles<E, DIM, true>), grid, dim3(256), 0, stream, p, (int)tiles, (int)items, (int)per_xcd);
+    hipLaunchKernelGGL((kv_attn_tiles<E, DIM, WAVES, true>), grid, block, 0, stream, p, (int)tiles, (int)items, (int)per_xcd);
   else
-    hipLaunchKernelGGL((kv_attn_tiles<E, DIM, false>), grid, dim3(256), 0, stream, p, (int)tiles, (int)items, (int)per_xcd);
+    hipLaunchKernelGGL((kv_attn_tiles<E, DIM, WAVES, false>), grid, block, 0, stream, p, (int)tiles, (int)items, (int)per_xcd);
   return hipGetLastError();
 }
 
 template <typename E, int DIM>
 hipError_t launch_any(const KvAttnParams& p, int rows, hipStream_t stream) {
-  const hipError_t e = rows == 16 ? launch_rows<E, DIM, 1>(p, stream) : launch_tiles<E, DIM>(p, stream);
+  hipError_t e = hipErrorInvalidValue;
+  if (rows == 16) e = launch_rows<E, DIM, 1>(p, stream);
+  else if (rows == 128) e = launch_tiles<E, DIM, 4>(p, stream);
+  else if constexpr (DIM == 128) e = launch_tiles<E, DIM, 8>(p, stream);
   if (e != hipSuccess || p.splits == 1) return e;
   const int64_t wgs = (p.tokens * p.q_heads + 3) / 4;
   if (wgs > 0x7fffffff) return hipErrorInvalidValue;
@@ -936,9 +972,9 @@ KvAttnPlan kv_attn_plan(int64_t tokens, int requests, int q_heads, int kv_heads,
   const int group = q_heads / kv_heads;
   const int64_t mean = (tokens * group + requests - 1) / requests;
   KvAttnPlan plan;
-  plan.rows = mean <= 16 ? 16 : 128;
+  plan.rows = mean <= 16 ? 16 : mean <= 128 || dim != 128 ? 128 : 256;
   const double wgs = (double)((mean + plan.rows - 1) / plan.rows) * requests * kv_heads;
-  const double slots = plan.rows == 16 ? 768 : 512;
+  const double slots = plan.rows == 16 ? 768 : plan.rows == 128 ? 512 : 256;
   const double work_us = plan.rows == 16 ? 2.0 * requests * max_kv * kv_heads * dim / 5.5e6
                                          : 4.0 * tokens * max_kv * q_heads * dim / 1e9;
   const double part_us = 2.0 * tokens * q_heads * (dim + 2) * sizeof(float) / 4.5e6;  // written and read
