@@ -514,19 +514,29 @@ struct KvTile {
   static constexpr int NP = 4 * HF / WAVES;  // 1 KB pieces of K, and of V, that a wave brings of a tile
   static constexpr int KBYTES = 64 * DIM * 2, VBYTES = KBYTES;
   static_assert(NP >= 1, "every wave brings a piece");
+  // With one piece a wave there are registers to fetch a tile two steps before it is widened, and LDS to hold K three
+  // tiles deep, so that a step's first operands are read before the barrier that opens it; else one and two.
+  static constexpr int SETS = NP == 1 ? 2 : 1, KBUFS = NP == 1 ? 3 : 2;
 };
 
 constexpr int kAhead = 4;  // LDS reads in flight
+
+// Workgroup barrier behind this wave's LDS writes, with its last N LDS reads still in flight (LDS answers in order).
+template <int N>
+__device__ __forceinline__ void barrier_lds() {
+  __builtin_amdgcn_s_waitcnt(0xC07F | (N << 8));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // UNI: pages of 64 tokens and more, so that a tile has one page and its number stays in scalar registers.
 template <typename E, int DIM, int WAVES, bool UNI>
 __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, int tiles, int items, int per_xcd) {
   using C = KvTile<DIM, WAVES>;
   constexpr int KS = C::KS, DT = C::DT, NP = C::NP;
-  // Tiles are fetched a step before they are widened; with eight waves two steps, for a wave then holds half as much.
-  constexpr int SETS = WAVES == 8 ? 2 : 1;
+  constexpr int SETS = C::SETS, KBUFS = C::KBUFS;
   using vec8 = typename E::vec8;
-  __shared__ __attribute__((aligned(1024))) unsigned char Ks[2][C::KBYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char Ks[KBUFS][C::KBYTES];
   __shared__ __attribute__((aligned(1024))) unsigned char Vs[2][C::VBYTES];
   // Workgroup n runs on XCD n % 8, which takes a contiguous run of (head, part of the keys, tile): the tiles of a
   // head sweep the same keys at the same time and find them in the XCD's L2.
@@ -594,8 +604,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
   // Pieces of a tile that this thread brings: of 16-key tile kt of K row m's 16 channels 64 f + 16 g .. of NP halves f
   // from kf on; of V channels 16 (NP wave + n) + m, keys 16 g .. + 15.  Their pages are looked up a step ahead.
   const int kt = wave & 3, kf = WAVES == 8 ? wave >> 2 : 0;
-  const int k_lane = ((UNI ? 16 * (m >> 2) : 0) + 4 * kt + (m & 3)) * DIM + 64 * kf + 16 * g;
-  const int v_lane = ((16 * NP * wave + m) << c.page_log2) + (UNI ? 16 * g : 0);
+  const uint32_t k_lane = ((UNI ? 16 * (m >> 2) : 0) + 4 * kt + (m & 3)) * DIM + 64 * kf + 16 * g;
+  const uint32_t v_lane = ((16 * NP * wave + m) << c.page_log2) + (UNI ? 16 * g : 0);
   auto k_key = [&](int tile) { return UNI ? tile * 64 : tile * 64 + 16 * (m >> 2); };
   auto v_key = [&](int tile) { return UNI ? tile * 64 : tile * 64 + 16 * g; };
   uint4 kr[SETS][NP], vr[SETS][NP];
@@ -615,7 +625,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
   };
   // Half u of piece n, widened, into buffer b.
   auto stage_k = [&](int b, int n, int u, const uint4& x) {
-    vec8* d = reinterpret_cast<vec8*>(Ks[b] + (kt * KS + 2 * (kf + n) + u) * 1024) + lane;
+    vec8* d = reinterpret_cast<vec8*>(Ks[0] + b * C::KBYTES + (kt * KS + 2 * (kf + n) + u) * 1024) + lane;
     d[0] = u ? widen<E>(x.z, x.w) : widen<E>(x.x, x.y);
   };
   auto stage_v = [&](int b, int n, int u, const uint4& x) {
@@ -715,68 +725,83 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
 
   part_tiles(tb, wb);
   if (wb < we) {
-    // Scores run a tile ahead of the weights and sums: at the top of a step K of tile + 1 and V of tile are in LDS and s
-    // holds the tile's scores.  The scores of the next tile and the weights of this one need nothing of each other, nor
+    // Scores run a tile ahead of the weights and sums: in step `tile` s holds the tile's scores, V of the tile and K of the
+    // next KBUFS - 1 are in LDS.  The scores of the next tile and the weights of this one need nothing of each other, nor
     // do the sums and the widening of what comes next: matrix and vector instructions run in each other's time.
-    // Page of the lane's key j, or with UNI of the tile's: from a vector register that holds the next 64 table entries
-    // (scalar loads would make every wait for an LDS read a wait for all of them).
-    int held = 0, held_at = -64;
-    auto look = [&](int j) -> int {
-      const int e = j >> c.page_log2;
-      if constexpr (UNI) {
-        if (e >= held_at + 64) {
-          held_at = e;
-          held = table[min(e + lane, (we * 64 - 1) >> c.page_log2)];
-          asm volatile("" : "+v"(held));  // waited for here, not at every use below, which would wait for the tiles' loads
-        }
-        return __builtin_amdgcn_readlane(held, e - held_at);
-      } else {
-        return table[e];
-      }
-    };
+    // The step widens K of tile + KBUFS and V of tile + 1 from one register set, and fetches the same SETS - 1 tiles on.
+    constexpr int KN = KBUFS + SETS - 1, VN = SETS;
     auto clip = [&](int tile) { return min(tile, we - 1); };
     auto as_is = [](const uint4& w) { return w; };
+    // Page of the lane's key j.  With UNI it is the tile's: the number comes through a vector load all the same (a
+    // scalar one would make every wait for an LDS read a wait for it), is read from one lane a step later, and K's
+    // serves V KN - VN steps after.
+    auto look = [&](int j) { return table[j >> c.page_log2]; };
+    auto uni = [](int id) { return UNI ? __builtin_amdgcn_readfirstlane(id) : id; };
     f32x4_t sa[4][2], sb[4][2];
     float sc, vf, inv, mx[2];
     auto scales = [&](int set) {
-      const int ke = page_exp(UNI ? __builtin_amdgcn_readfirstlane(ke_n[set]) : ke_n[set]);
-      const int ve = page_exp(UNI ? __builtin_amdgcn_readfirstlane(ve_n[set]) : ve_n[set]);
+      const int ke = page_exp(uni(ke_n[set])), ve = page_exp(uni(ve_n[set]));
       sc = p.scale * exp2_int(ke);
       vf = (float)ve;
       inv = exp2_int(-ve);
     };
-    // Step `tile` widens K of tile + 2 and V of tile + 1 from its set, and fetches those SETS - 1 tiles on into the other.
-    constexpr int KN = SETS + 1;  // K's distance when it is fetched (V's: SETS)
-    int vid, kid;
-    auto look_next = [&](int tile) {  // pages of what step `tile` fetches
-      vid = look(v_key(clip(tile + SETS)));
-      kid = look(k_key(clip(tile + KN)));
-    };
-    fetch_k(0, wb, look(k_key(wb)));
-    fetch_v(0, wb, look(v_key(wb)));
+    auto k_id = [&](int tile) { return uni(look(k_key(clip(tile)))); };
+    auto v_id = [&](int tile) { return uni(look(v_key(clip(tile)))); };
+    fetch_k(0, wb, k_id(wb));
+    fetch_v(0, wb, v_id(wb));
     barrier_lds_reads_done();
     stage_all(0, kr[0], stage_k);
     stage_all(0, vr[0], stage_v);
     scales(0);
-    int id1v = look(v_key(clip(wb + 1)));
-    fetch_k(0, clip(wb + 1), look(k_key(clip(wb + 1))));
-    if constexpr (SETS == 2) {
-      fetch_v(1, clip(wb + 1), id1v);
-      fetch_k(1, clip(wb + 2), look(k_key(clip(wb + 2))));
+#pragma unroll
+    for (int n = 1; n < KBUFS; ++n) {
+      fetch_k(0, clip(wb + n), k_id(wb + n));
+      stage_all(n, kr[0], stage_k);
     }
-    look_next(wb);
-    if constexpr (SETS == 1) vid = id1v;
+    if constexpr (SETS == 2) {
+      fetch_v(1, clip(wb + 1), v_id(wb + 1));
+      fetch_k(1, clip(wb + KBUFS), k_id(wb + KBUFS));
+    }
+    // What step wb fetches: K of wb + KN (and, with UNI, the pages of the tiles between that and V's), V of wb + VN.
+    int kid = look(k_key(clip(wb + KN))), vid = look(v_key(clip(wb + VN)));
+    int mid[KN - VN];
+#pragma unroll
+    for (int n = 0; n < KN - VN; ++n) mid[n] = UNI ? k_id(wb + VN + n) : 0;
     barrier_lds_reads_done();
     scores(0, sa);
-    stage_all(1, kr[0], stage_k);
 #pragma unroll
     for (int q = 0; q < 2; ++q) mx[q] = lane_max<2>(sa, q, sc, vf);
+    // (KBUFS == 2: K of the tile after next goes where the scores were just read.)
+    uint4 first[kAhead];
+    int kb = 0;  // (tile - wb) % KBUFS
+    auto k_at = [&](int b) { return Ks[0] + b * C::KBYTES; };
+    auto k_read = [&](const unsigned char* at, int f) { return *(reinterpret_cast<const uint4*>(at + ((f % 4) * KS + f / 4) * 1024) + lane); };
+    if constexpr (KBUFS == 3) {
+#pragma unroll
+      for (int f = 0; f < kAhead; ++f) first[f] = k_read(k_at(1), f);
+    }
     barrier_lds_reads_done();
     auto step = [&](int tile, int b, f32x4_t (&s)[4][2], f32x4_t (&sn)[4][2]) {
       const int fs = SETS == 2 ? b : 0, ss = SETS == 2 ? b ^ 1 : 0;  // sets to fetch into, to widen from
-      fetch_k(fs, clip(tile + KN), kid);
-      fetch_v(fs, clip(tile + SETS), vid);
-      look_next(tile + 1);
+      const int kb1 = kb + 1 == KBUFS ? 0 : kb + 1, kb2 = kb1 + 1 == KBUFS ? 0 : kb1 + 1;
+      const unsigned char* k_src = k_at(kb1);
+      int kid1 = 0, vid1 = 0;
+      // The next step's page numbers are asked for before the tiles, whose loads then need not be waited for with them.
+      auto look_next = [&] {
+        kid1 = look(k_key(clip(tile + 1 + KN)));
+        if (!UNI) vid1 = look(v_key(clip(tile + 1 + VN)));
+      };
+      int last_id = 0;
+      auto fetch_next_k = [&] {
+        last_id = uni(kid);
+        fetch_k(fs, clip(tile + KN), last_id);
+      };
+      auto fetch_next_v = [&] { fetch_v(fs, clip(tile + VN), UNI ? mid[0] : vid); };
+      if constexpr (SETS == 1) {
+        fetch_next_k();
+        fetch_next_v();
+        look_next();
+      }
       raise_max<DT, 2>(mx, m_run, l_run, o);
       // One operand at a time, read kAhead operands before, and its two MFMAs; between them, first the weights of 32 / NF
       // scores, then a piece of the next tiles' codes widened and a share of the maxima.  The order is fixed
@@ -787,11 +812,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
       auto read = [&](int f) {
         if (f >= 2 * NF) return;
         const int v = f - NF;
-        fr[f] = f < NF ? *(reinterpret_cast<const uint4*>(Ks[b ^ 1] + ((f % 4) * KS + f / 4) * 1024) + lane)
-                       : *(reinterpret_cast<const uint4*>(Vs[b] + (2 * (v % DT) + v / DT) * 1024) + lane);
+        fr[f] = f < NF ? k_read(k_src, f) : *(reinterpret_cast<const uint4*>(Vs[b] + (2 * (v % DT) + v / DT) * 1024) + lane);
       };
 #pragma unroll
-      for (int f = 0; f < kAhead; ++f) read(f);
+      for (int f = 0; f < kAhead; ++f) {
+        if constexpr (KBUFS == 3) fr[f] = first[f];
+        else read(f);
+      }
       float off[2], sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int q = 0; q < 2; ++q) off[q] = vf - m_run[q] + kShift;
@@ -813,6 +840,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
           sum[q] += p0 + p1;
           asm volatile("" : "+v"(sum[q]));  // added here: sunk behind the loop, the sums would keep 32 weights in registers
         }
+        if constexpr (SETS == 2) {
+          if (f == 0) look_next();
+          if (f == NF / 4) fetch_next_k();
+          if (f == NF / 2) fetch_next_v();
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
       f16x8_t pf[2][2];
@@ -831,7 +863,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
         constexpr int EVERY = NF / (4 * NP);  // one half of a piece of K, then of V, every so many operands
         if (f % EVERY == EVERY - 1) {
           const int i = f / EVERY;
-          if (i < 2 * NP) stage_k(b, i / 2, i % 2, kr[ss][i / 2]);
+          if (i < 2 * NP) stage_k(kb, i / 2, i % 2, kr[ss][i / 2]);
           else stage_v(b ^ 1, i / 2 - NP, i % 2, vr[ss][i / 2 - NP]);
         }
 #pragma unroll
@@ -843,10 +875,23 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+      if constexpr (KBUFS == 3) {
+#pragma unroll
+        for (int f = 0; f < kAhead; ++f) first[f] = k_read(k_at(kb2), f);
+      }
       scales(ss);
 #pragma unroll
       for (int q = 0; q < 2; ++q) mx[q] = fmaf(mx[q], sc, vf);
-      barrier_lds_reads_done();
+      kid = kid1;
+      if (UNI) {
+#pragma unroll
+        for (int n = 0; n < KN - VN - 1; ++n) mid[n] = mid[n + 1];
+        mid[KN - VN - 1] = last_id;
+      } else {
+        vid = vid1;
+      }
+      kb = kb1;
+      barrier_lds<KBUFS == 3 ? kAhead : 0>();
     };
     auto finish = [&](int b, const f32x4_t (&s)[4][2]) {
       f16x8_t pf[2][2];
