@@ -166,6 +166,23 @@ def check(fn: str, status: int) -> None:
         raise PasaError(fn, status, msg)
 
 
+def on_stream(device, fn: str, *args) -> None:
+    """``call`` with ``device`` current and torch's current stream of it as the last argument."""
+    import torch
+    if torch.cuda.current_device() == device.index:
+        call(fn, *args, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            call(fn, *args, _raw_stream(device.index))
+
+
+def _raw_stream(index: int) -> int:
+    """The handle of torch's current stream on device ``index``, without making a Stream object (1.6 us) where it can."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return torch.cuda.current_stream(index).cuda_stream if raw is None else raw(index)
+
+
 def call(fn: str, *args) -> int:
     """Call an int-returning entry point and raise PasaError on a negative status."""
     rc = getattr(load(), fn)(*args)

@@ -62,6 +62,12 @@ __device__ __forceinline__ uint32_t first_bytes(int n) {
 // 0x80 in each byte that is e4m3's NaN (0x7f or 0xff).
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+// A word of codes with 0 in the place of each NaN.
+__device__ __forceinline__ uint32_t finite_bytes(uint32_t w) {
+  const uint32_t n = nan_bytes(w);
+  return w & ~(n | (n - (n >> 7)));
+}
+
 // The requests' first rows of q, clamped to the rows that there are.
 // (tokens * q_heads < 2^31: row numbers fit 32 bits.)
 __device__ __forceinline__ int first_token(const KvAttnParams& p, int r) {
@@ -69,23 +75,36 @@ __device__ __forceinline__ int first_token(const KvAttnParams& p, int r) {
   return min(max(p.cu_q[r], 0), (int)p.tokens);
 }
 
-// Tile `id` of the launch: request r (requests: the rows behind the last one), and its first row.  The tiles of a
-// request are numbered from floor(first row / TILE) + r, which leaves room for every request's last, part-filled one
-// without a sum over the requests before it.
+// Tile `id` of the launch: request r (requests: the rows behind the last one), its first token and rows, the tile's first
+// row, and the request's length.  The tiles of a request are numbered from floor(first row / TILE) + r, which leaves room
+// for every request's last, part-filled one without a sum over the requests before it.
+struct TileOf {
+  int r, tok0, rows, row0, raw_len;
+};
 template <int TILE>
-__device__ __forceinline__ int find_tile(const KvAttnParams& p, int id, int& tok0, int& rows, int& row0) {
-  int lo = 0, hi = p.requests + 1;
-  auto start = [&](int r) { return first_token(p, r) * p.group / TILE + r; };
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (start(mid) <= id) lo = mid;
-    else hi = mid;
+__device__ __forceinline__ TileOf find_tile(const KvAttnParams& p, int id) {
+  // The last request whose number is at or before id: 64 candidates at a time, one for each lane, which in the last round
+  // (the only one for up to 63 requests) also has its request's length.
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = p.requests + 1;
+  auto number = [&](int first, int r) { return first * p.group / TILE + r; };
+  while (n > 64) {
+    const int step = (n + 63) >> 6, at = lo + min(lane * step, n - 1);
+    const int before = max(__popcll(__ballot(lane * step < n && number(first_token(p, at), at) <= id)), 1) - 1;
+    lo += before * step;
+    n = min(step, n - before * step);
   }
-  tok0 = first_token(p, lo);
-  const int tok1 = lo == p.requests ? (int)p.tokens : max(first_token(p, lo + 1), tok0);
-  rows = (tok1 - tok0) * p.group;
-  row0 = (id - start(lo)) * TILE;
-  return lo;
+  const int at = min(lo + lane, p.requests);
+  const int first = first_token(p, at), len = p.lens[min(at, p.requests - 1)];
+  const int i = max(__popcll(__ballot(lane < n && number(first, at) <= id)), 1) - 1;
+  TileOf t;
+  t.r = lo + i;
+  t.tok0 = __builtin_amdgcn_readlane(first, i);
+  const int tok1 = t.r == p.requests ? (int)p.tokens : i < 63 ? __builtin_amdgcn_readlane(first, min(i + 1, 63)) : first_token(p, t.r + 1);
+  t.rows = (max(tok1, t.tok0) - t.tok0) * p.group;
+  t.row0 = (id - number(t.tok0, t.r)) * TILE;
+  t.raw_len = max(__builtin_amdgcn_readlane(len, i), 0);
+  return t;
 }
 
 // What position pos of a request of len keys sees: [sees_lo, sees_hi).
@@ -271,14 +290,17 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   return w & ~(n | (n - (n >> 15)));
 }
 
-// Few rows: a workgroup has 16 * NQ rows of one key head, its four waves take every fourth 64-key tile straight from
-// memory into registers, and their sums are joined in LDS.  blockIdx.z: a part of the keys.
+// ---- few rows --------------------------------------------------------------------
+// A workgroup has 16 * NQ rows of one key head; its eight waves take the 64-key tiles in turn, straight from memory into
+// registers, and their sums are joined in LDS.  blockIdx.z: a part of the keys.  Bound by the bytes of the keys: eight
+// waves a compute unit, each with a tile of 16 KB in flight, ask for more than HBM gives.
 template <typename E, int DIM, int NQ>
-__global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
+__global__ __launch_bounds__(512, 2) void kv_attn_rows(KvAttnParams p) {
+  constexpr int WAVES = 8;
   constexpr int TILE = 16 * NQ, KS = DIM / 32, DT = DIM / 16, HF = DIM / 64;
   using vec8 = typename E::vec8;
-  __shared__ float so[4][TILE][DIM + 4];
-  __shared__ float sm[4][TILE], sl[4][TILE];
+  __shared__ float so[WAVES][TILE][DIM + 4];
+  __shared__ float sm[WAVES][TILE], sl[WAVES][TILE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, g = lane >> 4;
@@ -286,29 +308,17 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
   const KvCache& c = p.c;
   const int page = 1 << c.page_log2;
 
-  int tok0, rows, row0;
-  const int r = find_tile<TILE>(p, blockIdx.x, tok0, rows, row0);
+  const TileOf tile_of = find_tile<TILE>(p, blockIdx.x);
+  const int r = tile_of.r, tok0 = tile_of.tok0, rows = tile_of.rows, row0 = tile_of.row0, raw_len = tile_of.raw_len;
   if (row0 < 0 || row0 >= rows) return;  // below 0: row starts that do not ascend
   if (r == p.requests) {
     zero_rows<TILE, DIM>(p, hk, z, tok0, rows, row0);
     return;
   }
-  const int raw_len = max(p.lens[r], 0);
   const int len = (int)min(min((int64_t)raw_len, p.max_kv), p.width << c.page_log2);
   const int64_t pos_base = (int64_t)raw_len - rows / p.group;
   const int32_t* table = p.tables + r * p.table_stride;
 
-  // This lane's rows: what they see is [lo, hi).
-  int64_t qtok[NQ];
-  int qhead[NQ], lo[NQ], hi[NQ];
-#pragma unroll
-  for (int t = 0; t < NQ; ++t) {
-    const int i = min(row0 + 16 * t + m, rows - 1), tok = i / p.group;
-    qhead[t] = hk * p.group + (i - tok * p.group);
-    lo[t] = sees_lo(p, pos_base + tok, len);
-    hi[t] = sees_hi(p, pos_base + tok, len);
-    qtok[t] = tok0 + tok;
-  }
   // What the tile's rows see together, in tiles of 64 keys; this part's share of them.
   const int last = min(row0 + TILE, rows) - 1;
   const int klo = sees_lo(p, pos_base + row0 / p.group, len), khi = sees_hi(p, pos_base + last / p.group, len);
@@ -316,9 +326,54 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
   const int per = (tile_hi - tile_lo + p.splits - 1) / p.splits;
   const int tb = min(tile_lo + z * per, tile_hi), te = min(tb + per, tile_hi);
 
-  vec8 qf[NQ][KS];
+  // Pages of the lane's K row and of its keys 16 g .. + 15 in a tile, -1 where there is none.
+  auto page_of = [&](int j) -> int {
+    const int id = table[min(j, len - 1) >> c.page_log2];
+    return j < len && (unsigned)id < (unsigned)c.num_pages ? id : -1;
+  };
+  // A tile's K is asked for when the scores of the one before are done, its V when the sums are, into the same registers.
+  int kid = -1, vid = -1, ke_n = 0, ve_n = 0;
+  bool here_n = false;
+  auto look_up = [&](int tile) {
+    kid = page_of(tile * 64 + 16 * (m >> 2));
+    vid = page_of(tile * 64 + 16 * g);
+  };
+  uint4 kr[4][HF], vr[DT];
+  auto fetch_k = [&](int tile) {
+    const int j = tile * 64 + 16 * (m >> 2);
+    const uint8_t* kp = c.k + ((((int64_t)max(kid, 0) * c.heads + hk) << c.page_log2) + (j & (page - 1)) + (m & 3)) * DIM + 16 * g;
 #pragma unroll
-  for (int t = 0; t < NQ; ++t) load_q<E, KS>(p, qtok[t], qhead[t], g, qf[t]);
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int f = 0; f < HF; ++f) kr[t][f] = *reinterpret_cast<const uint4*>(kp + 4 * t * DIM + 64 * f);
+  };
+  const uint8_t* vp = c.v;
+  auto fetch_v = [&](int tile) {
+    const int64_t at = (int64_t)max(vid, 0) * c.heads + hk;
+    vp = c.v + (((at * DIM) + m) << c.page_log2) + ((tile * 64 + 16 * g) & (page - 1));
+    here_n = vid >= 0;
+    ke_n = c.k_exp[at];
+    ve_n = c.v_exp[at];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) vr[dt] = *reinterpret_cast<const uint4*>(vp + ((16 * dt) << c.page_log2));
+  };
+  if (tb + wave < te) {
+    look_up(tb + wave);
+    fetch_k(tb + wave);
+    fetch_v(tb + wave);
+    if (tb + wave + WAVES < te) look_up(tb + wave + WAVES);
+  }
+
+  // This lane's rows: what they see is [lo, hi).
+  vec8 qf[NQ][KS];
+  int lo[NQ], hi[NQ];
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    const int i = min(row0 + 16 * t + m, rows - 1), tok = i / p.group;
+    lo[t] = sees_lo(p, pos_base + tok, len);
+    hi[t] = sees_hi(p, pos_base + tok, len);
+    load_q<E, KS>(p, tok0 + tok, hk * p.group + (i - tok * p.group), g, qf[t]);
+  }
 
   f32x4_t o[DT][NQ];
   float l_run[NQ], m_run[NQ];
@@ -330,30 +385,18 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
     for (int dt = 0; dt < DT; ++dt) o[dt][t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   }
 
-  // Page of key j, or -1.
-  auto page_of = [&](int j) -> int {
-    if (j >= len) return -1;
-    const int id = table[j >> c.page_log2];
-    return id >= 0 && id < c.num_pages ? id : -1;
+  // Bytes of the lane's keys jv .. + 15 that are the request's.
+  auto kept = [&](int jv, bool here) {
+    const int n = here ? min(max(len - jv, 0), 16) : 0;
+    return make_uint4(first_bytes(n), first_bytes(n - 4), first_bytes(n - 8), first_bytes(n - 12));
   };
-  const int64_t page_bytes = (int64_t)page * DIM;
+  uint32_t poison = 0u;
 
-  for (int tile = tb + wave; tile < te; tile += 4) {
-    const int j0 = tile * 64;
-    const int jk = j0 + 16 * (m >> 2), jv = j0 + 16 * g;
-    const int kid = max(page_of(jk), 0), vid = page_of(jv);
-    const bool here = vid >= 0;
-    const int64_t vat = (int64_t)max(vid, 0) * c.heads + hk;
-    const uint8_t* kp = c.k + ((int64_t)kid * c.heads + hk) * page_bytes + ((jk & (page - 1)) + (m & 3)) * DIM + 16 * g;
-    const uint8_t* vp = c.v + vat * page_bytes + m * page + (jv & (page - 1));
-    uint4 kr[4][HF], vr[DT];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int f = 0; f < HF; ++f) kr[t][f] = *reinterpret_cast<const uint4*>(kp + 4 * t * DIM + 64 * f);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) vr[dt] = *reinterpret_cast<const uint4*>(vp + 16 * dt * page);
-    const int ke = page_exp(c.k_exp[vat]), ve = page_exp(c.v_exp[vat]);
+  for (int tile = tb + wave; tile < te; tile += WAVES) {
+    const int jv = tile * 64 + 16 * g;
+    const bool here = here_n;
+    const int ke = page_exp(ke_n), ve = page_exp(ve_n);
+    const bool more = tile + WAVES < te;
 
     f32x4_t s[4][NQ];
 #pragma unroll
@@ -372,35 +415,32 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
         }
       }
 
-    // Keys that a row does not see.
+    if (more) fetch_k(tile + WAVES);
+
+    // Keys that a row does not see: key jv + e for e below a and from b on.  Codes behind the last key are whatever the
+    // page held: zero times them has to be zero.  So has zero times a NaN that the row does not see; the products run
+    // without NaN, and the outputs that one does reach become NaN behind the loop.
     bool all_seen = here;
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) all_seen = all_seen && lo[q] <= jv && jv + 16 <= hi[q];
-    const bool whole = __all(all_seen);
-    bool poison = false;
-    if (!whole) {
+    for (int q = 0; q < NQ; ++q) all_seen = all_seen & (lo[q] <= jv) & (jv + 16 <= hi[q]);
+    if (!__all(all_seen)) {
 #pragma unroll
-      for (int q = 0; q < NQ; ++q)
+      for (int q = 0; q < NQ; ++q) {
+        const int a = here ? lo[q] - jv : 16, b = here ? hi[q] - jv : 0;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = jv + 4 * t + i;
-            if (!here || j < lo[q] || j >= hi[q]) s[t][q][i] = -INFINITY;
-          }
-      // Codes behind the last key are whatever the page held: zero times them has to be zero.  A NaN among the
-      // request's own codes must not reach rows that do not see it.
-      const int nb = here ? min(max(len - jv, 0), 16) : 0;
-      uint32_t any = 0u;
+        for (int e = 0; e < 16; ++e) {
+          const float x = s[e >> 2][q][e & 3];
+          s[e >> 2][q][e & 3] = ((e >= a) & (e < b)) ? x : -INFINITY;
+        }
+      }
+      const uint4 keep = kept(jv, here);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        vr[dt].x &= first_bytes(nb);
-        vr[dt].y &= first_bytes(nb - 4);
-        vr[dt].z &= first_bytes(nb - 8);
-        vr[dt].w &= first_bytes(nb - 12);
-        any |= nan_bytes(vr[dt].x) | nan_bytes(vr[dt].y) | nan_bytes(vr[dt].z) | nan_bytes(vr[dt].w);
+        uint4& w = vr[dt];
+        w = make_uint4(w.x & keep.x, w.y & keep.y, w.z & keep.z, w.w & keep.w);
+        poison |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
+        w = make_uint4(finite_bytes(w.x), finite_bytes(w.y), finite_bytes(w.z), finite_bytes(w.w));
       }
-      poison = __any(any != 0u);
     }
     const float sc = p.scale * exp2_int(ke), inv = exp2_int(-ve);
     f16x8_t pf[2][NQ];
@@ -409,41 +449,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
     for (int q = 0; q < NQ; ++q) mx[q] = lane_max<NQ>(s, q, sc, (float)ve);
     raise_max<DT, NQ>(mx, m_run, l_run, o);
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      weights<NQ>(s, q, sc, (float)ve, inv, m_run[q], l_run[q], pf[0][q], pf[1][q]);
-    }
-    if (poison) {
-      // 1 at each NaN code times 1 at each key that the row sees: rows with a product above 0 are NaN there.
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        uint32_t w[4] = {vr[dt].x, vr[dt].y, vr[dt].z, vr[dt].w};
-        uint32_t ind[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t n = nan_bytes(w[e]);
-          w[e] &= ~(n | (n - (n >> 7)));     // 0xff over each NaN byte
-          ind[e] = (n >> 7) * 0x38u;         // e4m3's 1.0
-        }
-        vr[dt] = make_uint4(w[0], w[1], w[2], w[3]);
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-          f32x4_t hit = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            f16x8_t seen;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int j = jv + 8 * u + e;
-              seen[e] = (_Float16)(here && j >= lo[q] && j < hi[q] ? 1.f : 0.f);
-            }
-            hit = F16::mfma16(widen_f16(ind[2 * u], ind[2 * u + 1]), seen, hit);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (hit[i] > 0.f) o[dt][q][i] = __uint_as_float(0x7fc00000u);
-        }
-      }
-    }
+    for (int q = 0; q < NQ; ++q) weights<NQ>(s, q, sc, (float)ve, inv, m_run[q], l_run[q], pf[0][q], pf[1][q]);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const f16x8_t a0 = widen_f16(vr[dt].x, vr[dt].y), a1 = widen_f16(vr[dt].z, vr[dt].w);
@@ -451,6 +457,37 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
       for (int q = 0; q < NQ; ++q) {
         o[dt][q] = F16::mfma16(a0, pf[0][q], o[dt][q]);
         o[dt][q] = F16::mfma16(a1, pf[1][q], o[dt][q]);
+      }
+    }
+    if (more) {
+      fetch_v(tile + WAVES);
+      if (tile + 2 * WAVES < te) look_up(tile + 2 * WAVES);
+    }
+  }
+
+  // NaN among the values of tiles that not every row sees whole: 1 at each times 1 at each key that a row sees is above 0
+  // where it reaches the row.
+  if (__any(poison != 0u)) {
+    for (int tile = tb + wave; tile < te; tile += WAVES) {
+      look_up(tile);
+      fetch_v(tile);
+      const int jv = tile * 64 + 16 * g;
+      const uint4 keep = kept(jv, here_n);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        f16x8_t seen[2];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) seen[e >> 3][e & 7] = (_Float16)(here_n && jv + e >= lo[q] && jv + e < hi[q] ? 1.f : 0.f);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const uint4& w = vr[dt];  // e4m3's 1.0 in the place of each NaN
+          const uint32_t ind[4] = {(nan_bytes(w.x & keep.x) >> 7) * 0x38u, (nan_bytes(w.y & keep.y) >> 7) * 0x38u,
+                                   (nan_bytes(w.z & keep.z) >> 7) * 0x38u, (nan_bytes(w.w & keep.w) >> 7) * 0x38u};
+          f32x4_t hit = F16::mfma16(widen_f16(ind[0], ind[1]), seen[0], (f32x4_t){0.f, 0.f, 0.f, 0.f});
+          hit = F16::mfma16(widen_f16(ind[2], ind[3]), seen[1], hit);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[dt][q][i] = hit[i] > 0.f ? __uint_as_float(0x7fc00000u) : o[dt][q][i];
+        }
       }
     }
   }
@@ -467,7 +504,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
     for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(&so[wave][16 * q + m][16 * dt + 4 * g]) = o[dt][q];
   }
   __syncthreads();
-  for (int e = tid; e < TILE * DIM / 4; e += 256) {
+  for (int e = tid; e < TILE * DIM / 4; e += 64 * WAVES) {
     const int i = e / (DIM / 4), d = (e % (DIM / 4)) * 4;
     const int row = row0 + i;
     if (row >= rows) break;
@@ -475,11 +512,11 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows(KvAttnParams p) {
     const int head = hk * p.group + row % p.group;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w][i]);
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sm[w][i]);
     float l = 0.f;
     f32x4_t acc = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
+#pragma unroll 4
+    for (int w = 0; w < WAVES; ++w) {
       const float f = sm[w][i] == -INFINITY ? 0.f : fast_exp2(sm[w][i] - top);
       const f32x4_t x = *reinterpret_cast<const f32x4_t*>(&so[w][i][d]);
       l += f * sl[w][i];
@@ -549,14 +586,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
   const KvCache& c = p.c;
   const int page = 1 << c.page_log2;
 
-  int tok0, rows, row0;
-  const int r = find_tile<C::ROWS>(p, item - hz * tiles, tok0, rows, row0);
+  const TileOf tile_of = find_tile<C::ROWS>(p, tiles - 1 - (item - hz * tiles));  // with a causal mask the last have most to do
+  const int r = tile_of.r, tok0 = tile_of.tok0, rows = tile_of.rows, row0 = tile_of.row0, raw_len = tile_of.raw_len;
   if (row0 < 0 || row0 >= rows) return;
   if (r == p.requests) {
     zero_rows<C::ROWS, DIM>(p, hk, z, tok0, rows, row0);
     return;
   }
-  const int raw_len = max(p.lens[r], 0);
   const int len = (int)min(min((int64_t)raw_len, p.max_kv), p.width << c.page_log2);
   const int64_t pos_base = (int64_t)raw_len - rows / p.group;
   const int32_t* table = p.tables + r * p.table_stride;
@@ -940,30 +976,47 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
   }
 }
 
-// Join the parts of the keys: one wave a row.
+// Join the parts of the keys: one wave a row.  Lane z has part z's maximum and sum (there are at most 64).
 template <int DIM>
 __global__ __launch_bounds__(256) void kv_attn_join(KvAttnParams p) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t all = p.tokens * p.q_heads;
   if (row >= all) return;
   const int64_t tok = row / p.q_heads;
   const int head = (int)(row - tok * p.q_heads);
-  const bool behind = p.cu_q != nullptr && tok >= min(max((int64_t)p.cu_q[p.requests], (int64_t)0), p.tokens);
+  const bool behind = p.cu_q != nullptr && tok >= first_token(p, p.requests);
   if (behind && !p.zero_tail) return;
   constexpr int N = DIM / 64;
-  float top = -INFINITY, l = 0.f, acc[N];
+  float top = -INFINITY, l = 0.f, f = 0.f, acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.f;
   if (!behind) {
-    for (int z = 0; z < p.splits; ++z) top = fmaxf(top, p.part_ml[2 * (z * all + row)]);
-    for (int z = 0; z < p.splits; ++z) {
-      const float m = p.part_ml[2 * (z * all + row)], lz = p.part_ml[2 * (z * all + row) + 1];
-      if (lz == 0.f) continue;
-      const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);  // m is -inf beside a NaN l where NaN is all that a row sees
-      l += f * lz;
+    if (lane < p.splits) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (lane * all + row));
+      top = ml.x;
+      l = ml.y;
+    }
+    float most = top;
 #pragma unroll
-      for (int k = 0; k < N; ++k) acc[k] += f * p.part_o[(z * all + row) * DIM + N * lane + k];
+    for (int d = 32; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
+    // A part without keys has l = 0; its maximum is -inf, as beside a NaN l where NaN is all that a row sees.
+    f = top == -INFINITY ? 0.f : fast_exp2(top - most);
+    l = wave_sum(l == 0.f ? 0.f : f * l);
+    top = most;
+    const float* part = p.part_o + row * DIM + N * lane;
+    for (int z = 0; z < p.splits; z += 8) {
+      float x[8][N];
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[n][k] = part[min(z + n, p.splits - 1) * all * DIM + k];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const float fz = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), min(z + n, 63)));
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += z + n < p.splits ? fz * x[n][k] : 0.f;
+      }
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -975,9 +1028,9 @@ __global__ __launch_bounds__(256) void kv_attn_join(KvAttnParams p) {
 template <typename E, int DIM, int NQ>
 hipError_t launch_rows(const KvAttnParams& p, hipStream_t stream) {
   const int64_t tiles = p.tokens * p.group / (16 * NQ) + p.requests + 1;
-  if (tiles > 0x7fffffff || p.c.heads > 65535 || p.splits > 65535) return hipErrorInvalidValue;
+  if (tiles > 0x7fffffff || p.c.heads > 65535 || p.splits > 64) return hipErrorInvalidValue;
   const dim3 grid((unsigned)tiles, (unsigned)p.c.heads, (unsigned)p.splits);
-  hipLaunchKernelGGL((kv_attn_rows<E, DIM, NQ>), grid, dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((kv_attn_rows<E, DIM, NQ>), grid, dim3(512), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -999,6 +1052,7 @@ template <typename E, int DIM>
 hipError_t launch_any(const KvAttnParams& p, int rows, hipStream_t stream) {
   hipError_t e = hipErrorInvalidValue;
   if (rows == 16) e = launch_rows<E, DIM, 1>(p, stream);
+  else if (rows == 32) e = launch_rows<E, DIM, 2>(p, stream);
   else if (rows == 128) e = launch_tiles<E, DIM, 4>(p, stream);
   else if constexpr (DIM == 128) e = launch_tiles<E, DIM, 8>(p, stream);
   if (e != hipSuccess || p.splits == 1) return e;
@@ -1010,26 +1064,32 @@ hipError_t launch_any(const KvAttnParams& p, int rows, hipStream_t stream) {
 
 }  // namespace
 
-// Tile and parts of the keys, from the sizes that the host knows.  A tile of 16 rows is bound by the bytes of the keys,
-// one of 128 by the matrix units; both run in rounds of as many workgroups as the chip holds at once, and a part of the
-// keys more makes the last round shorter but its sums pass through memory.  The parts with the least time are taken.
+// Tile and parts of the keys, from the sizes that the host knows.  Tiles of 16 and 32 rows are bound by the bytes of the
+// keys, of 128 and 256 by the matrix units (rates of long runs, in us).  The workgroups run in rounds of as many as the
+// chip holds at once; more parts of the keys make the last round shorter, but a workgroup begins and ends for some us and
+// its sums pass through memory and a second launch.  Parts are added while that gains 3%: workgroups that sweep the same
+// keys at the same time share them in L2, and the more rounds there are the further they drift apart (3,600 tokens x
+// 75,600 of 40 heads: 6.46 ms whole, 5.30 in 2 parts, 5.44 in 4, 5.80 in 5).
 KvAttnPlan kv_attn_plan(int64_t tokens, int requests, int q_heads, int kv_heads, int dim, int64_t max_kv) {
   const int group = q_heads / kv_heads;
   const int64_t mean = (tokens * group + requests - 1) / requests;
   KvAttnPlan plan;
-  plan.rows = mean <= 16 ? 16 : mean <= 128 || dim != 128 ? 128 : 256;
-  const double wgs = (double)((mean + plan.rows - 1) / plan.rows) * requests * kv_heads;
-  const double slots = plan.rows == 16 ? 768 : plan.rows == 128 ? 512 : 256;
-  const double work_us = plan.rows == 16 ? 2.0 * requests * max_kv * kv_heads * dim / 5.5e6
-                                         : 4.0 * tokens * max_kv * q_heads * dim / 1e9;
-  const double part_us = 2.0 * tokens * q_heads * (dim + 2) * sizeof(float) / 4.5e6;  // written and read
-  const int64_t most = (max_kv + 255) / 256 < 64 ? (max_kv + 255) / 256 : 64;        // four tiles a part at least
+  plan.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 128 || dim != 128 ? 128 : 256;
   plan.splits = 1;
+  const bool few = plan.rows <= 32;
+  // Four tiles a wave at most: one launch (1 token to 1,560 of 12 heads: 15.6 us on the GPU, 10 in four parts and their
+  // join, but 19.7 us a call against 23, which is what the two launches cost the host).
+  if (few && max_kv <= 2048) return plan;
+  const double wgs = (double)((mean + plan.rows - 1) / plan.rows) * requests * kv_heads;
+  const double slots = plan.rows == 128 ? 512 : 256;
+  const double work_us = few ? 2.0 * requests * max_kv * kv_heads * dim / (plan.rows == 16 ? 5.5e6 : 3.6e6) : 4.0 * tokens * max_kv * q_heads * dim / 1.1e9;
+  const double part_us = 2.0 * tokens * q_heads * (dim + 2) * sizeof(float) / 4.5e6;  // written and read
+  const int64_t most = (max_kv + 511) / 512 < 64 ? (max_kv + 511) / 512 : 64;        // eight tiles a part at least
   double best = 0.0;
   for (int n = 1; n <= most; ++n) {
     const double used = wgs * n, rounds = ceil(used / slots);
-    const double t = work_us * rounds * slots / used + (n > 1 ? 4.0 + n * part_us : 0.0);
-    if (n == 1 || t < best) {
+    const double t = work_us * rounds * slots / used + (few ? 3.0 : 10.0) * rounds + (n > 1 ? 4.0 + n * part_us : 0.0);
+    if (n == 1 || t < 0.97 * best) {
       best = t;
       plan.splits = n;
     }

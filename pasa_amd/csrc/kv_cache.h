@@ -122,7 +122,7 @@ struct KvAttnParams {
   float* part_ml;   // [splits, tokens * q_heads, 2]
 };
 struct KvAttnPlan {
-  int rows;    // rows of a workgroup's tile
+  int rows;    // rows of a workgroup's tile: 16 or 32 (few), 128 or 256
   int splits;
 };
 KvAttnPlan kv_attn_plan(int64_t tokens, int requests, int q_heads, int kv_heads, int dim, int64_t max_kv);

@@ -88,8 +88,7 @@ def _call(device: torch.device, fn: str, *args) -> None:
     """The library's call with ``device`` current, on its current stream."""
     if device.type != "cuda":
         raise ValueError("the cache kernels need ROCm device tensors (there is no CPU path)")
-    with torch.cuda.device(device):
-        _lib.call(fn, *args, torch.cuda.current_stream(device).cuda_stream)
+    _lib.on_stream(device, fn, *args)
 
 
 def _check_ints(device, dtype=torch.int32, **ts) -> None:
@@ -151,10 +150,8 @@ def extend_block_tables(block_tables: torch.Tensor, lens: torch.Tensor, new_toke
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError(f"tokens {tokens} is negative")
-    # One allocation: cu_q, lens, num_free and the positions, each 32 bits.
-    ints = torch.empty(2 * R + 2 + tokens, dtype=torch.int32, device=dev)
-    cu_q, after, left, positions = ints[:R + 1], ints[R + 1:2 * R + 1], ints[2 * R + 1:2 * R + 2], ints[2 * R + 2:]
-    slots = torch.empty(tokens, dtype=torch.int64, device=dev)
+    cu_q, after, left, positions = lens.new_empty(2 * R + 2 + tokens).split((R + 1, R, 1, tokens))
+    slots = lens.new_empty(tokens, dtype=torch.int64)
     _call(dev, "pasa_block_tables", block_tables.data_ptr(), max(block_tables.stride(0), block_tables.shape[1]),
           block_tables.shape[1], lens.data_ptr(), new_tokens.data_ptr(), R, free_pages.data_ptr(), free_pages.numel(),
           num_free.data_ptr(), page_size, tokens, cu_q.data_ptr(), slots.data_ptr(), positions.data_ptr(),
@@ -245,7 +242,7 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, block_tables: torch.Tenso
         raise ValueError(f"max_kv_len {max_kv_len} is negative")
     max_kv = min(width * cache.page_size, 2 ** 31 - 1 if max_kv_len is None else int(max_kv_len))
     if out is None:
-        o = torch.empty(T, H, D, dtype=q.dtype, device=dev)
+        o = q.new_empty((T, H, D))
     else:
         o = out
         if o.shape != q.shape or o.dtype != q.dtype or o.device != dev or (o.numel() and D > 1 and o.stride(2) != 1):
@@ -254,9 +251,9 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, block_tables: torch.Tenso
             raise ValueError("cached_attention has no gradient: out must not require one")
         if _lib.shares_memory(o) or _meets(o, q):
             raise ValueError("out: its rows and heads must not share memory with each other or with q")
-    lse = torch.empty(T, H, dtype=torch.float32, device=dev) if return_lse else None
+    lse = q.new_empty((T, H), dtype=torch.float32) if return_lse else None
     need = _lib.load().pasa_kv8_attn_workspace_bytes(T, R, H, cache.heads, cache.k.shape[3], max_kv)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     args = _lib.Kv8Attn(q.data_ptr(), o.data_ptr(), None if lse is None else lse.data_ptr(), q.stride(0), q.stride(1),
                         o.stride(0), o.stride(1), block_tables.data_ptr(), max(block_tables.stride(0), width), width,
                         lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), T, R, H, max_kv,

@@ -87,22 +87,22 @@ def _rotate(q, k, positions, axes, inverse, out):
         raise ValueError("the rotary kernel needs ROCm device tensors (there is no CPU path)")
     q4 = _bshd(q)
     B, S, _, D = q4.shape
-    pos = positions if positions.dim() == 3 else positions.unsqueeze(1).expand(-1, B, -1)
+    pos = positions
 
     def tensor(x, y):
         x, y = _bshd(x), _bshd(y)
-        t = _lib.RopeTensor(x.data_ptr(), y.data_ptr())
-        t.in_stride[:] = x.stride()[:3]
-        t.out_stride[:] = y.stride()[:3]
-        t.heads = x.shape[2]
-        return ctypes.byref(t)
+        (xb, xs, xh, _), (yb, ys, yh, _) = x.stride(), y.stride()
+        return ctypes.byref(_lib.RopeTensor(x.data_ptr(), y.data_ptr(), (xb, xs, xh), (yb, ys, yh), x.shape[2]))
 
-    with torch.cuda.device(q.device):
-        _lib.call("pasa_rope_axes", tensor(q, out[0]), None if k is None else tensor(k, out[1]), pos.data_ptr(),
-                  _POS[pos.dtype], pos.stride(0), pos.stride(1), pos.stride(2), pos.shape[0], axes.inv_freq.data_ptr(),
-                  axes.axis.data_ptr(), axes.inv_freq.numel(), B, S, D, PAIRINGS[axes.pairing], int(inverse),
-                  _DTYPES[q.dtype], torch.cuda.current_stream(q.device).cuda_stream)
+    _lib.on_stream(q.device, "pasa_rope_axes", tensor(q, out[0]), None if k is None else tensor(k, out[1]), pos.data_ptr(),
+                   _POS[pos.dtype], *_pos_strides(positions), pos.shape[0], axes.inv_freq.data_ptr(), axes.axis.data_ptr(),
+                   axes.inv_freq.numel(), B, S, D, PAIRINGS[axes.pairing], int(inverse), _DTYPES[q.dtype])
     return out
+
+
+def _pos_strides(pos: torch.Tensor) -> Tuple[int, int, int]:
+    """Strides along axes, batch and sequence; one row of positions serves every batch."""
+    return pos.stride() if pos.dim() == 3 else (pos.stride(0), 0, pos.stride(1))
 
 
 def _new(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
