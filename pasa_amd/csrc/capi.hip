@@ -1021,6 +1021,9 @@ int pasa_kv8_append(const pasa_kv8_t* cache, const void* k, const void* v, const
   p.tok_stride[1] = v_token_stride;
   p.head_stride[0] = k_head_stride;
   p.head_stride[1] = v_head_stride;
+  const int64_t piece = dtype == PASA_DTYPE_F32 ? 4 : 8;  // elements in 16 bytes
+  for (int i = 0; i < 2; ++i)
+    p.vec[i] = ((uintptr_t)p.x[i] & 15u) == 0 && p.tok_stride[i] % piece == 0 && p.head_stride[i] % piece == 0;
   p.slots = slots;
   p.tokens = tokens;
   p.dtype = dtype;

@@ -87,6 +87,7 @@ struct KvAppendParams {
   const void* x[2];       // k, v
   int64_t tok_stride[2];  // elements
   int64_t head_stride[2];
+  bool vec[2];  // eight channels can be loaded in 16-byte pieces
   const int64_t* slots;
   int64_t tokens;
   int dtype;
