@@ -71,13 +71,14 @@ __global__ __launch_bounds__(256) void rope_axes_scalar(RopeAxesParams p) {
 }
 
 // 16 bytes at a time.  A wave takes a token, or a part of its heads: a lane has one 16-byte unit of a head's channels
-// (HALVES: two, whose channels are each other's pairs), 64 / units heads lie side by side in the wave, and the lane's
-// sines stay in registers for all heads that follow.
+// (HALVES: two, whose channels are each other's pairs), 64 / units heads lie side by side in the wave.  The lanes share
+// out the pairs' angles, and through LDS each gets the sines of its own, which stay in registers for all heads.
 template <typename T, bool HALVES>
 __global__ __launch_bounds__(256) void rope_axes_vec(RopeAxesParams p, int units, int parts) {
   constexpr int V = 16 / sizeof(T);
   constexpr int N = HALVES ? 2 : 1;  // 16-byte pieces of a lane
   constexpr int P = HALVES ? V : V / 2;
+  __shared__ float2 turn[4][kMaxPairs];
   const int lane = threadIdx.x & 63;
   const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int64_t n = wave / parts;
@@ -103,10 +104,14 @@ __global__ __launch_bounds__(256) void rope_axes_vec(RopeAxesParams p, int units
   };
   Piece d[kRows][N];
   load(p.t[0], first, d);
+  float2* mine = turn[threadIdx.x >> 6];
+  for (int j = lane; j < p.pairs; j += 64) mine[j] = turn_of(p, j, b, s);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's own: no barrier
+  __builtin_amdgcn_wave_barrier();
   float2 cs[P];
   if (turns) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) cs[i] = turn_of(p, HALVES ? c0 + i : (c0 >> 1) + i, b, s);
+    for (int i = 0; i < P; ++i) cs[i] = mine[(HALVES ? c0 : c0 >> 1) + i];
   }
   for (int w = 0; w < 2; ++w) {
     const RopeAxesTensor& x = p.t[w];
