@@ -192,6 +192,8 @@ def call(fn: str, *args) -> int:
 
 def shares_memory(t) -> bool:
     """Whether two elements of the tensor ``t`` may share memory."""
+    if t.is_contiguous():
+        return False
     reach = 1
     for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
         if stride < reach:

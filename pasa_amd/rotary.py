@@ -62,8 +62,9 @@ def grid_positions(frames: int, height: int, width: int, first_frame: int = 0, d
     return torch.stack([first_frame + t // (height * width), t // width % height, t % width])
 
 
-def _bshd(t: torch.Tensor) -> torch.Tensor:
-    return t if t.dim() == 4 else t.unsqueeze(0)
+def _tokens(t: torch.Tensor) -> Tuple[int, int]:
+    """Batch and sequence of a [B, S, heads, D] or [tokens, heads, D] tensor."""
+    return (1, t.shape[0]) if t.dim() == 3 else t.shape[:2]
 
 
 def _check_tensor(t: torch.Tensor, name: str) -> None:
@@ -85,24 +86,21 @@ def _rotate(q, k, positions, axes, inverse, out):
     """The launch: outputs ``out`` (one for each of q, k)."""
     if not q.is_cuda:
         raise ValueError("the rotary kernel needs ROCm device tensors (there is no CPU path)")
-    q4 = _bshd(q)
-    B, S, _, D = q4.shape
-    pos = positions
+    B, S = _tokens(q)
+    pos_stride = positions.stride()
+    if len(pos_stride) == 2:  # one row of positions serves every batch
+        pos_stride = (pos_stride[0], 0, pos_stride[1])
 
     def tensor(x, y):
-        x, y = _bshd(x), _bshd(y)
-        (xb, xs, xh, _), (yb, ys, yh, _) = x.stride(), y.stride()
-        return ctypes.byref(_lib.RopeTensor(x.data_ptr(), y.data_ptr(), (xb, xs, xh), (yb, ys, yh), x.shape[2]))
+        xs, ys = x.stride(), y.stride()
+        if len(xs) == 3:
+            xs, ys = (0,) + xs, (0,) + ys
+        return ctypes.byref(_lib.RopeTensor(x.data_ptr(), y.data_ptr(), xs[:3], ys[:3], x.shape[-2]))
 
-    _lib.on_stream(q.device, "pasa_rope_axes", tensor(q, out[0]), None if k is None else tensor(k, out[1]), pos.data_ptr(),
-                   _POS[pos.dtype], *_pos_strides(positions), pos.shape[0], axes.inv_freq.data_ptr(), axes.axis.data_ptr(),
-                   axes.inv_freq.numel(), B, S, D, PAIRINGS[axes.pairing], int(inverse), _DTYPES[q.dtype])
+    _lib.on_stream(q.device, "pasa_rope_axes", tensor(q, out[0]), None if k is None else tensor(k, out[1]), positions.data_ptr(),
+                   _POS[positions.dtype], *pos_stride, positions.shape[0], axes.inv_freq.data_ptr(), axes.axis.data_ptr(),
+                   axes.inv_freq.numel(), B, S, q.shape[-1], PAIRINGS[axes.pairing], int(inverse), _DTYPES[q.dtype])
     return out
-
-
-def _pos_strides(pos: torch.Tensor) -> Tuple[int, int, int]:
-    """Strides along axes, batch and sequence; one row of positions serves every batch."""
-    return pos.stride() if pos.dim() == 3 else (pos.stride(0), 0, pos.stride(1))
 
 
 def _new(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -147,7 +145,7 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
         _check_tensor(k, "k")
         if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1] or k.dtype != q.dtype:
             raise ValueError(f"k must have q's tokens, head dim and dtype, got {k.dtype} {tuple(k.shape)} for q {q.dtype} {tuple(q.shape)}")
-    B, S = (1, q.shape[0]) if q.dim() == 3 else q.shape[:2]
+    B, S = _tokens(q)
     if positions.dtype not in _POS:
         raise ValueError(f"positions: dtype {positions.dtype} is not int32, int64 or float32")
     if tuple(positions.shape[1:]) not in ((S,), (B, S)) or positions.dim() < 2:
