@@ -489,6 +489,8 @@ int pasa_kv8_append(const pasa_kv8_t* cache, const void* k, const void* v, const
                     int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
                     int dtype, void* stream);
 
+#define PASA_KV8_MAX_KEYS ((int64_t)0x7fffff00)
+
 /* One call of pasa_kv8_attn. */
 typedef struct {
   const void* q;                 /* [tokens, q_heads, head_dim] bf16 or fp16, channels contiguous   */
@@ -498,12 +500,12 @@ typedef struct {
   const int32_t* block_tables;   /* [requests, width], rows table_stride apart; -1: no page         */
   int64_t table_stride, width;
   const int32_t* lens;           /* [requests]: cached tokens, the new ones included                 */
-  const int32_t* cu_q;           /* [requests + 1]: first row of each request; NULL: tokens / requests each */
+  const int32_t* cu_q;           /* [requests + 1], ascending: first row of each request; NULL: tokens / requests each */
   int64_t tokens, requests, q_heads;
-  int64_t max_kv;                /* keys from here on are not looked at                             */
+  int64_t max_kv;                /* keys from here on are not looked at; at most PASA_KV8_MAX_KEYS  */
   int64_t window;                /* 0: none                                                         */
   int causal;
-  int zero_tail;                 /* rows behind the last request become 0 (lse: -inf); else left as they were */
+  int zero_tail;                 /* rows of no request (in front of the first, behind the last) become 0 (lse: -inf); else left as they were */
   int dtype;
   double scale;                  /* of the scores, in [1e-20, 1e20]                                 */
 } pasa_kv8_attn_t;

@@ -1036,6 +1036,8 @@ static int check_kv8_attn_sizes(int64_t tokens, int64_t requests, int64_t q_head
                 (long long)tokens, (long long)requests, (long long)q_heads, (long long)kv_heads, (long long)max_kv);
   if (requests > kMaxI32 / 2 || q_heads > kMaxGridY || tokens > kMaxI32 / q_heads)
     return fail(PASA_ERR_OVERFLOW, "pasa_kv8_attn: tokens=%lld of %lld heads, requests=%lld", (long long)tokens, (long long)q_heads, (long long)requests);
+  if (max_kv > PASA_KV8_MAX_KEYS)
+    return fail(PASA_ERR_OVERFLOW, "pasa_kv8_attn: max_kv=%lld (at most %lld)", (long long)max_kv, (long long)PASA_KV8_MAX_KEYS);
   return PASA_OK;
 }
 

@@ -80,6 +80,7 @@ __device__ __forceinline__ int first_token(const KvAttnParams& p, int r) {
 // for every request's last, part-filled one without a sum over the requests before it.
 struct TileOf {
   int r, tok0, rows, row0, raw_len;
+  int front;  // tile 0 only: the first request's first token
 };
 template <int TILE>
 __device__ __forceinline__ TileOf find_tile(const KvAttnParams& p, int id) {
@@ -104,6 +105,7 @@ __device__ __forceinline__ TileOf find_tile(const KvAttnParams& p, int id) {
   t.rows = (max(tok1, t.tok0) - t.tok0) * p.group;
   t.row0 = (id - number(t.tok0, t.r)) * TILE;
   t.raw_len = max(__builtin_amdgcn_readlane(len, i), 0);
+  t.front = __builtin_amdgcn_readlane(first, 0);  // (only request 0 has a number that tile 0 reaches)
   return t;
 }
 
@@ -131,16 +133,15 @@ __device__ __forceinline__ float row_lse(float top, float l) {
   return kLn2 * ((top + ((float)x - kShift)) + __log2f(frac));
 }
 
-// Rows behind the last request.
-template <int TILE, int DIM>
-__device__ __forceinline__ void zero_rows(const KvAttnParams& p, int hk, int z, int tok0, int rows, int row0) {
+// n of the rows of no request, from row0 of token tok0 on.
+template <int DIM>
+__device__ __forceinline__ void zero_rows(const KvAttnParams& p, int hk, int z, int tok0, int row0, int n) {
   if (!p.zero_tail || z != 0 || p.splits != 1) return;  // with parts, the join writes them
-  for (int e = threadIdx.x; e < TILE * DIM; e += blockDim.x) {
-    const int i = row0 + e / DIM;
-    if (i >= rows) break;
+  for (int64_t e = threadIdx.x; e < (int64_t)n * DIM; e += blockDim.x) {
+    const int i = row0 + (int)(e / DIM);
     const int64_t tok = tok0 + i / p.group;
     const int head = hk * p.group + i % p.group;
-    store_rowpart(p, tok, head, e % DIM, 0.f);
+    store_rowpart(p, tok, head, (int)(e % DIM), 0.f);
     if (e % DIM == 0 && p.lse) p.lse[tok * p.q_heads + head] = -INFINITY;
   }
 }
@@ -309,10 +310,11 @@ __global__ __launch_bounds__(512, 2) void kv_attn_rows(KvAttnParams p) {
   const int page = 1 << c.page_log2;
 
   const TileOf tile_of = find_tile<TILE>(p, blockIdx.x);
+  if (blockIdx.x == 0 && tile_of.front > 0) zero_rows<DIM>(p, hk, z, 0, 0, tile_of.front * p.group);
   const int r = tile_of.r, tok0 = tile_of.tok0, rows = tile_of.rows, row0 = tile_of.row0, raw_len = tile_of.raw_len;
   if (row0 < 0 || row0 >= rows) return;  // below 0: row starts that do not ascend
   if (r == p.requests) {
-    zero_rows<TILE, DIM>(p, hk, z, tok0, rows, row0);
+    zero_rows<DIM>(p, hk, z, tok0, row0, min(TILE, rows - row0));
     return;
   }
   const int len = (int)min(min((int64_t)raw_len, p.max_kv), p.width << c.page_log2);
@@ -539,11 +541,16 @@ __global__ __launch_bounds__(512, 2) void kv_attn_rows(KvAttnParams p) {
 }
 
 // ---- many rows --------------------------------------------------------------------
-// A workgroup has 128 rows of one key head, 32 a wave, and walks the keys in tiles of 64.  A tile's codes come from
-// memory once for the workgroup: each thread widens 16-byte pieces and writes them to LDS as the operands that the
-// waves' MFMAs read (1 KB pieces, lane after lane: no bank conflicts either way), while the tile before is computed.
-// Two buffers, one barrier a tile.  Widening once for 128 rows costs 32 conversions a thread and tile of 16-bit LDS
-// traffic; widening after the LDS read would cost each wave 128.
+// A workgroup has 128 rows of one key head, or 256 where there are as many and the head dim is 128, 32 a wave, and walks
+// the keys in tiles of 64.  A tile's codes come from memory once for the workgroup: each thread widens 16-byte pieces and
+// writes them to LDS as the operands that the waves' MFMAs read (1 KB pieces, lane after lane: no bank conflicts either
+// way).  Widening once for 256 rows costs a thread 32 conversions a tile; widening behind the LDS read would cost 256.
+// Bound by the SIMDs' issue: an MFMA of 16 cycles has 32 rows x 64 keys x 32 channels / 4, and between two of them go the
+// scale, exponential, sum, maximum and rounding of two scores (about 11 cycles at head dim 128, twice that at 64) and the
+// LDS reads.  3,600 tokens x 75,600 keys of 40 heads of 128 channels: 14.3 ms with 16-row tiles, 9.65 with 128 rows, 6.2
+// with 256 (half the LDS reads and widening a row) and the scores a tile ahead, 5.3 with K three tiles deep: 1.05 PFLOP/s,
+// where the chip's matrix products reach 1.37.  12 requests of 1,500 tokens, 32 heads of 64 channels, a causal window of
+// 4,096 on 6,000 keys: 0.26 ms, 0.62 PFLOP/s.
 template <int DIM, int WAVES>
 struct KvTile {
   static constexpr int ROWS = 32 * WAVES;
@@ -558,7 +565,8 @@ struct KvTile {
 
 constexpr int kAhead = 4;  // LDS reads in flight
 
-// Workgroup barrier behind this wave's LDS writes, with its last N LDS reads still in flight (LDS answers in order).
+// Workgroup barrier behind this wave's LDS writes, with its last N LDS reads still in flight (LDS answers in order; N
+// reads have to be there, behind the last write).
 template <int N>
 __device__ __forceinline__ void barrier_lds() {
   __builtin_amdgcn_s_waitcnt(0xC07F | (N << 8));
@@ -586,11 +594,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
   const KvCache& c = p.c;
   const int page = 1 << c.page_log2;
 
-  const TileOf tile_of = find_tile<C::ROWS>(p, tiles - 1 - (item - hz * tiles));  // with a causal mask the last have most to do
+  const int id = tiles - 1 - (item - hz * tiles);  // with a causal mask the last have most to do
+  const TileOf tile_of = find_tile<C::ROWS>(p, id);
+  if (id == 0 && tile_of.front > 0) zero_rows<DIM>(p, hk, z, 0, 0, tile_of.front * p.group);
   const int r = tile_of.r, tok0 = tile_of.tok0, rows = tile_of.rows, row0 = tile_of.row0, raw_len = tile_of.raw_len;
   if (row0 < 0 || row0 >= rows) return;
   if (r == p.requests) {
-    zero_rows<C::ROWS, DIM>(p, hk, z, tok0, rows, row0);
+    zero_rows<DIM>(p, hk, z, tok0, row0, min(C::ROWS, rows - row0));
     return;
   }
   const int len = (int)min(min((int64_t)raw_len, p.max_kv), p.width << c.page_log2);
@@ -817,7 +827,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
       for (int f = 0; f < kAhead; ++f) first[f] = k_read(k_at(1), f);
     }
     barrier_lds_reads_done();
-    auto step = [&](int tile, int b, f32x4_t (&s)[4][2], f32x4_t (&sn)[4][2]) {
+    // last: no step follows, so that nothing but LDS writes is in flight at the barrier, which waits for them.
+    auto step = [&](int tile, int b, f32x4_t (&s)[4][2], f32x4_t (&sn)[4][2], auto last) {
+      constexpr bool FIRST = KBUFS == 3 && !decltype(last)::value;
       const int fs = SETS == 2 ? b : 0, ss = SETS == 2 ? b ^ 1 : 0;  // sets to fetch into, to widen from
       const int kb1 = kb + 1 == KBUFS ? 0 : kb + 1, kb2 = kb1 + 1 == KBUFS ? 0 : kb1 + 1;
       const unsigned char* k_src = k_at(kb1);
@@ -911,7 +923,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (KBUFS == 3) {
+      if constexpr (FIRST) {
 #pragma unroll
         for (int f = 0; f < kAhead; ++f) first[f] = k_read(k_at(kb2), f);
       }
@@ -927,7 +939,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
         vid = vid1;
       }
       kb = kb1;
-      barrier_lds<KBUFS == 3 ? kAhead : 0>();
+      barrier_lds<FIRST ? kAhead : 0>();
     };
     auto finish = [&](int b, const f32x4_t (&s)[4][2]) {
       f16x8_t pf[2][2];
@@ -940,11 +952,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
     };
     int tile = wb;
     for (; tile + 2 < we; tile += 2) {
-      step(tile, 0, sa, sb);
-      step(tile + 1, 1, sb, sa);
+      step(tile, 0, sa, sb, std::false_type{});
+      step(tile + 1, 1, sb, sa, std::false_type{});
     }
     if (tile + 1 < we) {
-      step(tile, 0, sa, sb);
+      step(tile, 0, sa, sb, std::true_type{});
       finish(1, sb);
     } else {
       finish(0, sa);
@@ -985,13 +997,13 @@ __global__ __launch_bounds__(256) void kv_attn_join(KvAttnParams p) {
   if (row >= all) return;
   const int64_t tok = row / p.q_heads;
   const int head = (int)(row - tok * p.q_heads);
-  const bool behind = p.cu_q != nullptr && tok >= first_token(p, p.requests);
-  if (behind && !p.zero_tail) return;
+  const bool none = p.cu_q != nullptr && (tok >= first_token(p, p.requests) || tok < first_token(p, 0));  // of no request
+  if (none && !p.zero_tail) return;
   constexpr int N = DIM / 64;
   float top = -INFINITY, l = 0.f, f = 0.f, acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.f;
-  if (!behind) {
+  if (!none) {
     if (lane < p.splits) {
       const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (lane * all + row));
       top = ml.x;

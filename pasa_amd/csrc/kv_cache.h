@@ -114,7 +114,7 @@ struct KvAttnParams {
   int64_t max_kv;   // keys from here on are not looked at
   int64_t window;   // 0: none
   int causal;
-  int zero_tail;    // rows behind the last request are set to zero
+  int zero_tail;    // rows of no request are set to zero
   int q_vec, o_vec; // rows of q / o are 16-byte aligned
   float scale;      // softmax scale * log2 e
   int f16;          // q and o are fp16, else bf16

@@ -25,6 +25,7 @@ _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch
 PAGE_SIZES = (16, 32, 64, 128)
 EXP_MIN, EXP_MAX = -50, 50
 MAX_TABLE_REQUESTS = 4096
+MAX_KEYS = 0x7fffff00  # of a request
 
 
 @dataclass
@@ -200,7 +201,7 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, block_tables: torch.Tenso
     """Softmax attention of q [tokens, q_heads, head_dim] (bf16 or fp16) to the cache.
 
     block_tables: int32 [requests, width]; lens: int32 [requests], cached tokens with the new ones; cu_q: int32
-    [requests + 1], first row of each request's new tokens, or None if each has tokens / requests of them.  New token i
+    [requests + 1], ascending, first row of each request's new tokens, or None if each has tokens / requests of them.  New token i
     of n is at position lens - n + i.  It sees every cached key, or with ``causal`` those up to its own, or with
     ``window`` the last ``window`` up to its own (and, without ``causal``, those behind it).  A table entry of -1 hides
     its page, as where early frames were given back.  Rows that see no key are 0.  q_heads is a multiple of the
@@ -208,7 +209,7 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, block_tables: torch.Tenso
 
     ``scale``: of the scores, default head_dim ** -0.5.  ``max_kv_len``: a bound of lens known on the host (default:
     the table's width); the work is split by it, and keys from there on are not read.  ``out``: where the result
-    goes; rows behind the last request are left as they were there, and 0 in a new tensor.  ``return_lse``: also the
+    goes; rows of no request (in front of the first, behind the last) stay as they were there, and are 0 in a new tensor.  ``return_lse``: also the
     natural logarithm of each row's sum of exponentials, fp32 [tokens, q_heads] (-inf where a row sees nothing)."""
     st = cache._struct()
     dev = cache.k.device
@@ -240,7 +241,9 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, block_tables: torch.Tenso
         raise ValueError(f"window {window} must be at least 1")
     if max_kv_len is not None and max_kv_len < 0:
         raise ValueError(f"max_kv_len {max_kv_len} is negative")
-    max_kv = min(width * cache.page_size, 2 ** 31 - 1 if max_kv_len is None else int(max_kv_len))
+    max_kv = width * cache.page_size if max_kv_len is None else min(width * cache.page_size, int(max_kv_len))
+    if max_kv > MAX_KEYS:
+        raise ValueError(f"a request of {max_kv} keys: at most {MAX_KEYS} are taken (max_kv_len bounds them)")
     if out is None:
         o = q.new_empty((T, H, D))
     else:

@@ -139,7 +139,11 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
     contiguous ([B, heads, S, D] tensors are passed as ``t.transpose(1, 2)``).  positions: [axes, S] (for every
     batch) or [axes, B, S], int32, int64 or fp32.  The angle positions[axis[i]] * inv_freq[i] is reduced in fp64;
     the rotation is fp32, rounded once.  ``inverse`` turns back.  ``inplace`` writes q and k themselves (no
-    gradient).  Returns (q, k)."""
+    gradient).  Returns (q, k).
+
+    Under graph capture with gradients, leaves must have no living graph from before: torch ties a leaf's gradient to
+    the stream of its first graph, and waiting for that stream breaks the capture.  Where such a graph came from here,
+    the call is refused; ``q.detach().requires_grad_()`` is a leaf of its own."""
     _check_tensor(q, "q")
     if k is not None:
         _check_tensor(k, "k")
@@ -175,9 +179,23 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
         _rotate(q, k, positions, axes, inverse, (q, k))
         return q, k
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        held = [_leaf_node(t) for t in (q, k) if t is not None and t.requires_grad and t.is_leaf]
         out = _RopeAxes.apply(q, k, positions, axes, inverse)
+        del held  # (the graph has the nodes now)
         return (out, None) if k is None else out
     return tuple(_rotate(q, k, positions, axes, inverse, (_new(q), _new(k))))
+
+
+def _leaf_node(t: torch.Tensor):
+    """The node that takes leaf ``t``'s gradient, marked with the stream that this module first met it on.  It lives as
+    long as some graph of the leaf does."""
+    node = torch.autograd.graph.get_gradient_edge(t).node
+    if t.is_cuda:
+        stream = _lib._raw_stream(t.device.index)
+        if node.metadata.setdefault("rope_axes stream", stream) != stream and torch.cuda.is_current_stream_capturing():
+            raise ValueError("rope_axes under graph capture: a graph of this leaf made on another stream is alive; give "
+                             "the call t.detach().requires_grad_()")
+    return node
 
 
 def _slices_of_one(q: torch.Tensor, k: torch.Tensor) -> bool:

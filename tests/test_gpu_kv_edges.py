@@ -1,0 +1,88 @@
+"""Calls at the edges of what the cache's attention and the rotary embedding are documented to take: rows in front of
+the first request, captured backward passes beside living graphs, pieces that do not line up."""
+import pytest
+import torch
+
+from pasa_amd.kv_cache import cached_attention
+from pasa_amd.rotary import RotaryAxes, rope_axes
+from test_gpu_kv_attention import check, make
+from test_gpu_rotary import close as against, make as values
+
+pytestmark = pytest.mark.gpu
+
+
+# (heads of q, of k, head dim, new, cached): rows of one tile, split rows, tiles of 128 and of 256 rows, those split.
+@pytest.mark.parametrize("Hq,Hk,D,new,kv", [
+    (2, 2, 128, [1, 1], [40, 70]), (4, 1, 64, [3, 9], [90, 700]), (2, 1, 128, [2, 1], [9000, 8000]),
+    (8, 1, 64, [40, 60], [300, 200]), (8, 1, 128, [90, 80], [500, 130]), (8, 1, 128, [70, 60], [6000, 5000])])
+@pytest.mark.parametrize("front", [1, 37])
+def test_rows_in_front_of_the_first_request(device, Hq, Hk, D, new, kv, front):
+    c, q, tables, kv, cu = make(device, kv, new, Hq, Hk, D, 64, torch.bfloat16, seed=front)
+    pad = torch.full((front, Hq, D), float("nan"), dtype=q.dtype, device=device)
+    q = torch.cat([pad, q, pad])
+    cu = [n + front for n in cu]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
+    torch.full((64, *q.shape), 7.0, dtype=q.dtype, device=device)  # what a new tensor finds in its memory
+    o, lse = cached_attention(q, c, i32(tables), i32(kv), i32(cu), causal=True, return_lse=True)
+    out = torch.full_like(q, 3.0)
+    cached_attention(q, c, i32(tables), i32(kv), i32(cu), causal=True, out=out)
+    torch.cuda.synchronize()
+    for rows in (slice(0, front), slice(cu[-1], None)):
+        assert bool((o[rows] == 0).all()) and bool((lse[rows] == -float("inf")).all())
+        assert bool((out[rows] == 3).all())
+    mine = slice(cu[0], cu[-1])
+    assert torch.equal(out[mine], o[mine])
+    want, _ = check((c, q[mine].contiguous(), tables, kv, [n - front for n in cu]), f"front {front}", causal=True)
+    # Another place of the rows in their tiles: another running maximum, and p rounded at another point.
+    assert torch.allclose(o[mine].float(), want.float(), rtol=2.0 ** -6, atol=2.0 ** -6 * float(want.float().abs().max()))
+
+
+def test_captured_gradient_beside_a_living_graph(device):
+    axes = RotaryAxes.video(64, device=device)
+    pos = torch.randint(0, 5000, (3, 33), dtype=torch.int32).to(device)
+    q, k = values((2, 33, 4, 64), torch.float16).requires_grad_(), values((2, 33, 2, 64), torch.float16, 1).requires_grad_()
+    gq, gk = values(q.shape, q.dtype, 2), values(k.shape, k.dtype, 3)
+    alive = rope_axes(q, k, pos, axes)
+    with pytest.raises(ValueError, match="graph of this leaf"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            rope_axes(q, k, pos, axes)
+    torch.cuda.synchronize()
+    q1, k1 = q.detach().requires_grad_(), k.detach().requires_grad_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = rope_axes(q1, k1, pos, axes)
+        grads = torch.autograd.grad(out, (q1, k1), (gq, gk))
+    for i in range(3):
+        pos.copy_(torch.randint(0, 5000, (3, 33), dtype=torch.int32).to(device))
+        with torch.no_grad():
+            q.mul_(1.01)
+            gk.mul_(0.99)
+        eager = rope_axes(q, k, pos, axes)
+        want = torch.autograd.grad(eager, (q, k), (gq, gk))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((*out, *grads), (*eager, *want)):
+            assert torch.equal(a, b), i
+    assert alive[0].requires_grad
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("pairing", ["interleaved", "halves"])
+@pytest.mark.parametrize("T,H,D,dims", [(1, 1, 8, (8,)), (1, 70, 128, (44, 42, 42)), (5, 3, 96, (32, 32)), (9000, 3, 64, (16, 8, 8)),
+                                        (8193, 1, 32, (16, 16)), (3, 2, 256, (256,)), (7, 9, 48, (20, 28)), (7, 9, 48, (20, 22))])
+def test_whole_pieces_and_others(device, dtype, pairing, T, H, D, dims):
+    """16-byte pieces, and the same values an element off them."""
+    axes = RotaryAxes.sections(dims, pairing=pairing, device=device)
+    pos = torch.randint(0, 3000, (len(dims), T), dtype=torch.int32).to(device)
+    x = values((T, H, D), dtype, T)
+    whole, k = rope_axes(x, x[:, :1], pos, axes)
+    close = lambda y, x, *a, **kw: against(y[None], x[None], *a, **kw)
+    close(whole, x, pos, axes, inverse=False, what="whole pieces")
+    close(k, x[:, :1], pos, axes, inverse=False, what="whole pieces, k")
+    room = torch.empty(T * H * D + 1, dtype=dtype, device=device)
+    off = room[1:].view(T, H, D)
+    off.copy_(x)
+    close(rope_axes(off, None, pos, axes)[0], x, pos, axes, inverse=False, what="an element off")
+    rope_axes(off, None, pos, axes, inplace=True)
+    close(off, x, pos, axes, inverse=False, what="an element off, in place")
