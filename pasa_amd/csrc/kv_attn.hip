@@ -241,19 +241,12 @@ __device__ __forceinline__ int page_exp(int e) { return min(max(e, kKvExpMin), k
 // 0x8000 in each 16-bit half that is an infinity or NaN (among widened codes: NaN).
 __device__ __forceinline__ uint32_t nan_halves(uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
 
-// A tile in LDS that not every row sees whole: a NaN among its values must not reach rows that do not see its key.
-// Where the tile holds one, the outputs that it does reach become NaN: 1 at each NaN times 1 at each key that the row
-// sees is above 0 there.  The products themselves then run on the values without NaN (finite_halves).
+// A tile in LDS that not every row sees whole and that holds a NaN among its values, which must not reach rows that do not
+// see its key.  The outputs that it does reach become NaN: 1 at each NaN times 1 at each key that the row sees is above 0
+// there.  The products themselves then run on the values without NaN (finite_halves).
 template <int DT>
 __device__ __forceinline__ void poison_step(const unsigned char* vs, int lane, bool here, int jv, const int (&lo)[2], const int (&hi)[2],
                                             f32x4_t (&o)[DT][2]) {
-  uint32_t any = 0u;
-#pragma unroll 2
-  for (int f = 0; f < 2 * DT; ++f) {
-    const uint4 w = *(reinterpret_cast<const uint4*>(vs + f * 1024) + lane);
-    any |= nan_halves(w.x) | nan_halves(w.y) | nan_halves(w.z) | nan_halves(w.w);
-  }
-  if (!__any(any != 0u)) return;
   uint64_t hits = 0u;  // bit 8 dt + 4 q + i
 #pragma unroll 1
   for (int dt = 0; dt < DT; ++dt) {
@@ -583,6 +576,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
   using vec8 = typename E::vec8;
   __shared__ __attribute__((aligned(1024))) unsigned char Ks[KBUFS][C::KBYTES];
   __shared__ __attribute__((aligned(1024))) unsigned char Vs[2][C::VBYTES];
+  __shared__ int nan_tile;  // the last tile, of those seen in part, that held a NaN among its values
   // Workgroup n runs on XCD n % 8, which takes a contiguous run of (head, part of the keys, tile): the tiles of a
   // head sweep the same keys at the same time and find them in the XCD's L2.
   const int slot = blockIdx.x >> 3, item = (blockIdx.x & 7) * per_xcd + slot;
@@ -656,11 +650,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
   auto v_key = [&](int tile) { return UNI ? tile * 64 : tile * 64 + 16 * g; };
   uint4 kr[SETS][NP], vr[SETS][NP];
   int ke_n[SETS], ve_n[SETS];  // exponents of the lane's keys 16 g .. + 15
-  auto fetch_k = [&](int set, int tile, int id) {
+  auto load_k = [&](uint4 (&to)[NP], int tile, int id) {
     const uint8_t* at = c.k + ((((int64_t)id * c.heads + hk) << c.page_log2) + (k_key(tile) & (page - 1))) * DIM + k_lane;
 #pragma unroll
-    for (int n = 0; n < NP; ++n) kr[set][n] = *reinterpret_cast<const uint4*>(at + 64 * n);
+    for (int n = 0; n < NP; ++n) to[n] = *reinterpret_cast<const uint4*>(at + 64 * n);
   };
+  auto fetch_k = [&](int set, int tile, int id) { load_k(kr[set], tile, id); };
   auto fetch_v = [&](int set, int tile, int id) {
     const int64_t row = (int64_t)id * c.heads + hk;
     const uint8_t* at = c.v + ((row * DIM) << c.page_log2) + (v_key(tile) & (page - 1)) + v_lane;
@@ -709,6 +704,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
       }
   };
 
+  auto as_is = [](const uint4& w) { return w; };
+
   // Tiles that some row sees in part, or whose pages are not all there: one at a time.
   auto part_tiles = [&](int t0, int t1) {
     if (t0 >= t1) return;
@@ -720,40 +717,65 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
       lo[q] = sees_lo(p, pos_base + tok, len);
       hi[q] = sees_hi(p, pos_base + tok, len);
     }
-    for (int tile = t0; tile < t1; ++tile) {
-      auto page_of = [&](int j) -> int {
-        const int id = j < len ? table[j >> c.page_log2] : -1;
-        return (unsigned)id < (unsigned)c.num_pages ? id : -1;
-      };
-      const int vid = page_of(v_key(tile));
-      const bool here = vid >= 0;
-      const int jv = tile * 64 + 16 * g;
-      fetch_k(0, tile, max(page_of(k_key(tile)), 0));
+    auto page_of = [&](int j) -> int {
+      const int id = j < len ? table[j >> c.page_log2] : -1;
+      return (unsigned)id < (unsigned)c.num_pages ? id : -1;
+    };
+    // A tile is fetched while the one before is computed, its page numbers a tile before that.
+    int kid = page_of(k_key(t0)), vid = page_of(v_key(t0));
+    bool here_n = false;
+    auto fetch = [&](int tile) {
+      here_n = vid >= 0;
+      fetch_k(0, tile, max(kid, 0));
       fetch_v(0, tile, max(vid, 0));
+      if (tile + 1 < t1) {
+        kid = page_of(k_key(tile + 1));
+        vid = page_of(v_key(tile + 1));
+      }
+    };
+    fetch(t0);
+    if (tid == 0) nan_tile = -1;
+    for (int tile = t0; tile < t1; ++tile) {
+      const bool here = here_n;
+      const int jv = tile * 64 + 16 * g;
       const int nb = here ? min(max(len - jv, 0), 16) : 0;  // codes behind the last key are whatever the page held
 #pragma unroll
       for (int n = 0; n < NP; ++n) {
         uint4& x = vr[0][n];
         x = make_uint4(x.x & first_bytes(nb), x.y & first_bytes(nb - 4), x.z & first_bytes(nb - 8), x.w & first_bytes(nb - 12));
       }
+      const int ke = page_exp(ke_n[0]), ve = page_exp(ve_n[0]);
+      uint32_t nan = 0u;
+#pragma unroll
+      for (int n = 0; n < NP; ++n) nan |= nan_bytes(vr[0][n].x) | nan_bytes(vr[0][n].y) | nan_bytes(vr[0][n].z) | nan_bytes(vr[0][n].w);
       barrier_lds_reads_done();
       stage_all(0, kr[0], stage_k);
       stage_all(0, vr[0], stage_v);
+      if (nan) nan_tile = tile;
+      if (tile + 1 < t1) fetch(tile + 1);
       barrier_lds_reads_done();
-      if (wrow >= rows) continue;  // (of the whole wave) nothing to compute, but the other waves' tiles to bring
-      f32x4_t s[4][2];
-      scores(0, s);
+      // Key jv + e is hidden from row tile q for e below a[q] and from b[q] on.
+      int a[2], b[2];
+      bool some = false, whole = true;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        // Key jv + e is hidden for e below a and from b on.
-        const int a = here ? lo[q] - jv : 16, b = here ? hi[q] - jv : 0;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float x = s[e >> 2][q][e & 3];
-          s[e >> 2][q][e & 3] = ((e >= a) & (e < b)) ? x : -INFINITY;
-        }
+        a[q] = here ? lo[q] - jv : 16;
+        b[q] = here ? hi[q] - jv : 0;
+        some = some | (max(a[q], 0) < min(b[q], 16));
+        whole = whole & (a[q] <= 0) & (b[q] >= 16);
       }
-      const int ke = page_exp(ke_n[0]), ve = page_exp(ve_n[0]);
+      if (wrow >= rows || !__any(some)) continue;  // the wave has no row here, but the other waves' tiles to bring
+      f32x4_t s[4][2];
+      scores(0, s);
+      if (!__all(whole)) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float x = s[e >> 2][q][e & 3];
+            s[e >> 2][q][e & 3] = ((e >= a[q]) & (e < b[q])) ? x : -INFINITY;
+          }
+      }
       const float sc = p.scale * exp2_int(ke), vf = (float)ve, inv = exp2_int(-ve);
       f16x8_t pf[2][2];
       float mx[2];
@@ -764,8 +786,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
       for (int q = 0; q < 2; ++q) {
         weights<2>(s, q, sc, vf, inv, m_run[q], l_run[q], pf[0][q], pf[1][q]);
       }
-      poison_step<DT>(Vs[0], lane, here, jv, lo, hi, o);
-      pv(0, pf, [](const uint4& w) { return make_uint4(finite_halves(w.x), finite_halves(w.y), finite_halves(w.z), finite_halves(w.w)); });
+      if (__builtin_amdgcn_readfirstlane(nan_tile) != tile) {
+        pv(0, pf, as_is);
+      } else {
+        poison_step<DT>(Vs[0], lane, here, jv, lo, hi, o);
+        pv(0, pf, [](const uint4& w) { return make_uint4(finite_halves(w.x), finite_halves(w.y), finite_halves(w.z), finite_halves(w.w)); });
+      }
     }
   };
 
@@ -777,7 +803,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
     // The step widens K of tile + KBUFS and V of tile + 1 from one register set, and fetches the same SETS - 1 tiles on.
     constexpr int KN = KBUFS + SETS - 1, VN = SETS;
     auto clip = [&](int tile) { return min(tile, we - 1); };
-    auto as_is = [](const uint4& w) { return w; };
     // Page of the lane's key j.  With UNI it is the tile's: the number comes through a vector load all the same (a
     // scalar one would make every wait for an LDS read a wait for it), is read from one lane a step later, and K's
     // serves V KN - VN steps after.
@@ -791,28 +816,30 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attn_tiles(KvAttnParams p, i
       vf = (float)ve;
       inv = exp2_int(-ve);
     };
-    auto k_id = [&](int tile) { return uni(look(k_key(clip(tile)))); };
-    auto v_id = [&](int tile) { return uni(look(v_key(clip(tile)))); };
-    fetch_k(0, wb, k_id(wb));
-    fetch_v(0, wb, v_id(wb));
-    barrier_lds_reads_done();
-    stage_all(0, kr[0], stage_k);
-    stage_all(0, vr[0], stage_v);
-    scales(0);
+    // All that step wb finds in LDS and in its registers is asked for at once, the page numbers first.
+    int ks[KN + 1], vs[VN + 1];
 #pragma unroll
-    for (int n = 1; n < KBUFS; ++n) {
-      fetch_k(0, clip(wb + n), k_id(wb + n));
-      stage_all(n, kr[0], stage_k);
-    }
+    for (int n = 0; n <= KN; ++n) ks[n] = look(k_key(clip(wb + n)));
+#pragma unroll
+    for (int n = 0; n <= VN; ++n) vs[n] = UNI ? ks[n] : look(v_key(clip(wb + n)));
+    uint4 k0[KBUFS][NP];
+#pragma unroll
+    for (int n = 0; n < KBUFS; ++n) load_k(k0[n], clip(wb + n), uni(ks[n]));
+    fetch_v(0, wb, uni(vs[0]));
     if constexpr (SETS == 2) {
-      fetch_v(1, clip(wb + 1), v_id(wb + 1));
-      fetch_k(1, clip(wb + KBUFS), k_id(wb + KBUFS));
+      fetch_v(1, clip(wb + 1), uni(vs[1]));
+      fetch_k(1, clip(wb + KBUFS), uni(ks[KBUFS]));
     }
     // What step wb fetches: K of wb + KN (and, with UNI, the pages of the tiles between that and V's), V of wb + VN.
-    int kid = look(k_key(clip(wb + KN))), vid = look(v_key(clip(wb + VN)));
+    int kid = ks[KN], vid = vs[VN];
     int mid[KN - VN];
 #pragma unroll
-    for (int n = 0; n < KN - VN; ++n) mid[n] = UNI ? k_id(wb + VN + n) : 0;
+    for (int n = 0; n < KN - VN; ++n) mid[n] = UNI ? uni(ks[VN + n]) : 0;
+    barrier_lds_reads_done();
+#pragma unroll
+    for (int n = 0; n < KBUFS; ++n) stage_all(n, k0[n], stage_k);
+    stage_all(0, vr[0], stage_v);
+    scales(0);
     barrier_lds_reads_done();
     scores(0, sa);
 #pragma unroll
