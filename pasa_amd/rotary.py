@@ -179,23 +179,21 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
         _rotate(q, k, positions, axes, inverse, (q, k))
         return q, k
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        held = [_leaf_node(t) for t in (q, k) if t is not None and t.requires_grad and t.is_leaf]
         out = _RopeAxes.apply(q, k, positions, axes, inverse)
-        del held  # (the graph has the nodes now)
+        _check_leaves(out if k is None else out[0], q.device)
         return (out, None) if k is None else out
     return tuple(_rotate(q, k, positions, axes, inverse, (_new(q), _new(k))))
 
 
-def _leaf_node(t: torch.Tensor):
-    """The node that takes leaf ``t``'s gradient, marked with the stream that this module first met it on.  It lives as
-    long as some graph of the leaf does."""
-    node = torch.autograd.graph.get_gradient_edge(t).node
-    if t.is_cuda:
-        stream = _lib._raw_stream(t.device.index)
-        if node.metadata.setdefault("rope_axes stream", stream) != stream and torch.cuda.is_current_stream_capturing():
+def _check_leaves(out: torch.Tensor, device) -> None:
+    """Mark the nodes that take the leaves' gradients with the stream that this module first met them on (a node lives as
+    long as some graph of its leaf does), and refuse a capture beside a graph that was made on another one."""
+    stream = _lib._raw_stream(device.index)
+    for node, _ in out.grad_fn.next_functions:
+        if hasattr(node, "variable") and node.metadata.setdefault("rope_axes stream", stream) != stream and \
+                torch.cuda.is_current_stream_capturing():
             raise ValueError("rope_axes under graph capture: a graph of this leaf made on another stream is alive; give "
                              "the call t.detach().requires_grad_()")
-    return node
 
 
 def _slices_of_one(q: torch.Tensor, k: torch.Tensor) -> bool:
