@@ -8,9 +8,9 @@
 //   code = e4m3(x * 2 ** -e), to nearest, ties to even; what is not finite is stored as NaN
 // and where e rises, the page's other codes are scaled by 2 ** (old e - e).  A run at offset 0 begins the page anew.
 //
-// Bound by HBM: 2 bytes in and 1 out of each value.  A thread's item is four tokens x eight channels, and the workgroup
-// has as many threads as a page has items, so that a run stays in registers between the maximum and the codes (a step
-// of single tokens has one wave to each; what does not fit is read twice).  k goes out as 8 bytes a token, v as words of
+// Bound by HBM: 2 bytes in and 1 out of each value (10,800 tokens x 40 heads x 128 channels: 84 us, 3.9 TB/s; single
+// values at a time, 623).  A thread's item is four tokens x eight channels, and the workgroup
+// has as many threads as a page has items, so that a run stays in registers between the maximum and the codes.  k goes out as 8 bytes a token, v as words of
 // four tokens, which is the way round it lies in the cache; runs of 16 tokens and more pass through LDS so that its rows
 // leave in 16-byte pieces.  16-bit values are compared and converted two at a time as they lie in memory.
 #include <type_traits>
@@ -110,7 +110,8 @@ struct Raw {
 // An item's largest magnitude as the bits of its type (in both halves of the word for a 16-bit one): as unsigned
 // numbers they are in the magnitudes' order, infinity and NaN above all others.
 template <typename T>
-__device__ __forceinline__ uint32_t top_bits(const Raw<T> (&r)[4], uint32_t top) {
+__device__ __forceinline__ uint32_t top_bits(const Raw<T> (&r)[4]) {
+  uint32_t top = 0u;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -160,30 +161,144 @@ __device__ __forceinline__ uint32_t codes_across(const Raw<T> (&r)[4], int i, in
   }
 }
 
-// blockIdx.x: the runs that begin among `window` tokens; y: the head; z: k or v.
+// The run of n tokens from token t on, at slot s and those behind it.  ALL: by the whole workgroup, else by one wave.
+template <typename T, bool ALL>
+__device__ __forceinline__ void append_run(const KvAppendParams& p, int h, int is_v, int64_t t, int64_t s, int n, float* wave_max, uint32_t* vt) {
+  const int tid = ALL ? threadIdx.x : threadIdx.x & 63, threads = ALL ? blockDim.x : 64;
+  const T* x = (const T*)p.x[is_v] + h * p.head_stride[is_v];
+  const int64_t tok_stride = p.tok_stride[is_v];
+  const bool vec = p.vec[is_v];
+  int8_t* exps = is_v ? p.c.v_exp : p.c.k_exp;
+  uint8_t* codes = is_v ? p.c.v : p.c.k;
+  const int page = 1 << p.c.page_log2, off = (int)(s & (page - 1));
+  const int D = p.c.head_dim, dim = p.c.dim, chunks = dim >> 3, chunks_log2 = dim == 128 ? 4 : 3;
+
+  // Item (pg, c): positions 4 pg .. + 3 of the page, channels 8 c .. + 7.
+  const int pg0 = off >> 2, items = (((off + n + 3) >> 2) - pg0) << chunks_log2;
+  // One item a thread at most: the threads are a page's items, or the run is short enough for a wave.
+  const int pos = 4 * (pg0 + (tid >> chunks_log2)), d0 = 8 * (tid & (chunks - 1));
+  Raw<T> raw[4];
+  {
+    const T* from = x + (t + pos - off) * tok_stride;
+#pragma unroll
+    for (int k = 0; k < 4; ++k, from += tok_stride) {
+      const int j = pos + k - off;
+      if (tid < items && j >= 0 && j < n) raw[k].load(from, d0, D, vec);
+      else raw[k].zero();
+    }
+  }
+  const int64_t at = (s >> p.c.page_log2) * p.c.heads + h;
+  const int had = off == 0 ? kKvExpMin : min(max((int)exps[at], kKvExpMin), kKvExpMax);
+  float most = from_bits<T>(top_bits<T>(raw));
+  const bool odd = !(most < INFINITY);  // something is not finite: it does not count
+  if (__any(odd)) {
+    most = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = fabsf(raw[k].at(e));
+        most = a < INFINITY ? fmaxf(most, a) : most;
+      }
+  }
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) most = fmaxf(most, __shfl_xor(most, m, 64));
+  bool careless;
+  if constexpr (ALL) {
+    if ((tid & 63) == 0) wave_max[tid >> 6] = most;
+    careless = !__syncthreads_or(odd);
+    for (int w = 0; w < threads / 64; ++w) most = fmaxf(most, wave_max[w]);
+  } else {
+    careless = !__any(odd);
+  }
+  const int e_new = max(had, exponent_of(most));
+  const bool careful = !careless || e_new == kKvExpMax;
+  uint8_t* out = codes + at * ((int64_t)page * dim);
+  if (tid == 0) exps[at] = (int8_t)e_new;  // (every thread has read it: the barrier above, or its wave's own order)
+  if (off != 0 && e_new != had) {
+    const float f = exp2_int(had - e_new);
+    uint32_t* words = reinterpret_cast<uint32_t*>(out);
+    for (int e = tid; e < page * dim / 4; e += threads) {
+      const int pos = is_v ? 4 * e & (page - 1) : 4 * e / dim;
+      const uint32_t mine = is_v ? bytes_in(pos, off, off + n) : pos >= off && pos < off + n ? 0xffffffffu : 0u;
+      if (mine != 0xffffffffu) {
+        // The run's own bytes of the word are written below, after a barrier.
+        const uint32_t old = words[e], now = rescaled4(old, f, mine);
+        if (now != old) words[e] = now;
+      }
+    }
+    if constexpr (ALL) {
+      __syncthreads();
+    } else {
+      __threadfence_block();  // the wave's stores arrive before those that follow
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  const bool through_lds = ALL && is_v && n >= 16;
+  const int row_words = page / 4 + 1;
+  if (tid < items) {
+    if (!is_v) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j = pos + k - off;
+        if (j < 0 || j >= n) continue;
+        *reinterpret_cast<uint2*>(out + (pos + k) * dim + d0) =
+            make_uint2(codes_along<T>(raw[k], 0, e_new, careful), codes_along<T>(raw[k], 1, e_new, careful));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t w = codes_across<T>(raw, i, e_new, careful);
+        if (through_lds) {
+          vt[(d0 + i) * row_words + (pos >> 2)] = w;
+        } else {
+          uint8_t* to = out + (d0 + i) * page + pos;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (pos + k >= off && pos + k < off + n) to[k] = (uint8_t)(w >> (8 * k));
+        }
+      }
+    }
+  }
+  if (through_lds) {
+    __syncthreads();
+    // 16 positions of a channel at a time; the first and last of the run may be cut.
+    const int u0 = off >> 4, units = ((off + n + 15) >> 4) - u0;
+    for (int e = tid; e < units * dim; e += threads) {
+      const int d = e / units, pos = 16 * (u0 + e - d * units);
+      const uint32_t* from = vt + d * row_words + (pos >> 2);
+      uint8_t* to = out + d * page + pos;
+      if (pos >= off && pos + 16 <= off + n) {
+        *reinterpret_cast<uint4*>(to) = make_uint4(from[0], from[1], from[2], from[3]);
+      } else {
+        for (int k = max(off - pos, 0); k < min(off + n - pos, 16); ++k) to[k] = (uint8_t)(from[k >> 2] >> (8 * (k & 3)));
+      }
+    }
+  }
+}
+
+// blockIdx.x: the runs that begin among `window` tokens; y: the head; z: k or v.  Runs of up to 64 items (one of a lane's)
+// are the waves', one each; the workgroup takes the longer ones together.
 template <typename T>
-__global__ __launch_bounds__(kMaxThreads) void kv_append(KvAppendParams p, int window) {
+__global__ __launch_bounds__(kMaxThreads, sizeof(T) == 4 ? 4 : 6) void kv_append(KvAppendParams p, int window) {
   __shared__ int64_t slots[64 + kMaxPage + 1];  // of tokens t0 - 1 ..
   __shared__ float wave_max[kMaxThreads / 64];
-  __shared__ uint32_t vt[128 * (kMaxPage / 4 + 1)];  // v's codes, a word more to a row: rows start in other banks
+  __shared__ uint64_t long_runs;
+  extern __shared__ uint32_t vt[];  // v's codes, dim rows of page / 4 words and one more: rows start in other banks
   const int tid = threadIdx.x, lane = tid & 63, threads = blockDim.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = blockIdx.y, is_v = blockIdx.z;
   const int page = 1 << p.c.page_log2;
   const int64_t t0 = (int64_t)blockIdx.x * window;
   const int64_t t1 = min(p.tokens, t0 + window);
   const int64_t end = min(p.tokens, t1 + page);
   const int64_t limit = (int64_t)p.c.num_pages << p.c.page_log2;
+  if (tid == 0) long_runs = 0u;
   for (int64_t t = t0 - 1 + tid; t < end; t += threads) {
     const int64_t s = t < 0 ? -2 : p.slots[t];
     slots[t - (t0 - 1)] = s < 0 || s >= limit ? -2 : s;
   }
   __syncthreads();
-  const T* x = (const T*)p.x[is_v] + h * p.head_stride[is_v];
-  const int64_t tok_stride = p.tok_stride[is_v];
-  const bool vec = p.vec[is_v];
-  int8_t* exps = is_v ? p.c.v_exp : p.c.k_exp;
-  uint8_t* codes = is_v ? p.c.v : p.c.k;
-  const int D = p.c.head_dim, dim = p.c.dim, chunks = dim >> 3, chunks_log2 = dim == 128 ? 4 : 3;
 
   // A token begins a run unless the one before it has the slot before, in the same page.
   uint64_t starts;
@@ -193,116 +308,29 @@ __global__ __launch_bounds__(kMaxThreads) void kv_append(KvAppendParams p, int w
     const int64_t s = in ? slots[i] : -2;
     starts = __ballot(s >= 0 && !(slots[in ? i - 1 : 0] == s - 1 && (s & (page - 1)) != 0));
   }
-  for (; starts != 0u; starts &= starts - 1) {
-    const int i = __builtin_ctzll(starts) + 1;
+  // The length of the run at token t0 + i - 1: how many of the next tokens have the next slots.
+  auto length = [&](int i) {
     const int64_t t = t0 + i - 1, s = slots[i];
     const int off = (int)(s & (page - 1));
-    // Its length: how many of the next tokens have the next slots.
     auto follows = [&](int k) { return off + k < page && t + k < end && slots[i + k] == s + k; };
     const uint64_t m0 = __ballot(follows(1 + lane)), m1 = __ballot(follows(65 + lane));
-    const int n = 1 + (~m0 ? __builtin_ctzll(~m0) : 64 + (~m1 ? __builtin_ctzll(~m1) : 64));
-
-    // Item (pg, c): positions 4 pg .. + 3 of the page, channels 8 c .. + 7.
-    const int pg0 = off >> 2, items = (((off + n + 3) >> 2) - pg0) << chunks_log2;
-    Raw<T> raw[4];
-    auto load = [&](int item) {
-      const int pos = 4 * (pg0 + (item >> chunks_log2)), d0 = 8 * (item & (chunks - 1));
-      const T* from = x + (t + pos - off) * tok_stride;
-#pragma unroll
-      for (int k = 0; k < 4; ++k, from += tok_stride) {
-        const int j = pos + k - off;
-        if (item < items && j >= 0 && j < n) raw[k].load(from, d0, D, vec);
-        else raw[k].zero();
-      }
-    };
-    const int64_t at = (s >> p.c.page_log2) * p.c.heads + h;
-    const int had = off == 0 ? kKvExpMin : min(max((int)exps[at], kKvExpMin), kKvExpMax);
-    uint32_t top = 0u;
-    for (int item = tid; item < items; item += threads) {
-      load(item);
-      top = top_bits<T>(raw, top);
-    }
-    float most = from_bits<T>(top);
-    const bool odd = !(most < INFINITY);  // something is not finite: it does not count
-    if (__any(odd)) {
-      most = 0.f;
-      for (int item = tid; item < items; item += threads) {
-        if (items > threads) load(item);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float a = fabsf(raw[k].at(e));
-            most = a < INFINITY ? fmaxf(most, a) : most;
-          }
-      }
-    }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) most = fmaxf(most, __shfl_xor(most, m, 64));
-    if (lane == 0) wave_max[tid >> 6] = most;
-    const bool careless = !__syncthreads_or(odd);
-    for (int w = 0; w < threads / 64; ++w) most = fmaxf(most, wave_max[w]);
-    const int e_new = max(had, exponent_of(most));
-    const bool careful = !careless || e_new == kKvExpMax;
-    uint8_t* out = codes + at * ((int64_t)page * dim);
-    if (tid == 0) exps[at] = (int8_t)e_new;  // (every thread has read it: the barrier above)
-    if (off != 0 && e_new != had) {
-      const float f = exp2_int(had - e_new);
-      uint32_t* words = reinterpret_cast<uint32_t*>(out);
-      for (int e = tid; e < page * dim / 4; e += threads) {
-        const int pos = is_v ? 4 * e & (page - 1) : 4 * e / dim;
-        const uint32_t mine = is_v ? bytes_in(pos, off, off + n) : pos >= off && pos < off + n ? 0xffffffffu : 0u;
-        if (mine != 0xffffffffu) {
-          // The run's own bytes of the word are written below, after a barrier.
-          const uint32_t old = words[e], now = rescaled4(old, f, mine);
-          if (now != old) words[e] = now;
-        }
-      }
-      __syncthreads();
-    }
-    const bool through_lds = is_v && n >= 16;
-    const int row_words = page / 4 + 1;
-    for (int item = tid; item < items; item += threads) {
-      const int pos = 4 * (pg0 + (item >> chunks_log2)), d0 = 8 * (item & (chunks - 1));
-      if (items > threads) load(item);
-      if (!is_v) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int j = pos + k - off;
-          if (j < 0 || j >= n) continue;
-          *reinterpret_cast<uint2*>(out + (pos + k) * dim + d0) =
-              make_uint2(codes_along<T>(raw[k], 0, e_new, careful), codes_along<T>(raw[k], 1, e_new, careful));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t w = codes_across<T>(raw, i, e_new, careful);
-          if (through_lds) {
-            vt[(d0 + i) * row_words + (pos >> 2)] = w;
-          } else {
-            uint8_t* to = out + (d0 + i) * page + pos;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (pos + k >= off && pos + k < off + n) to[k] = (uint8_t)(w >> (8 * k));
-          }
-        }
-      }
-    }
-    if (through_lds) {
-      __syncthreads();
-      // 16 positions of a channel at a time; the first and last of the run may be cut.
-      const int u0 = off >> 4, units = ((off + n + 15) >> 4) - u0;
-      for (int e = tid; e < units * dim; e += threads) {
-        const int d = e / units, pos = 16 * (u0 + e - d * units);
-        const uint32_t* from = vt + d * row_words + (pos >> 2);
-        uint8_t* to = out + d * page + pos;
-        if (pos >= off && pos + 16 <= off + n) {
-          *reinterpret_cast<uint4*>(to) = make_uint4(from[0], from[1], from[2], from[3]);
-        } else {
-          for (int k = max(off - pos, 0); k < min(off + n - pos, 16); ++k) to[k] = (uint8_t)(from[k >> 2] >> (8 * (k & 3)));
-        }
-      }
-    }
+    return 1 + (~m0 ? __builtin_ctzll(~m0) : 64 + (~m1 ? __builtin_ctzll(~m1) : 64));
+  };
+  int turn = 0;
+  for (uint64_t left = starts; left != 0u; left &= left - 1) {
+    if (turn++ % (threads / 64) != wave) continue;
+    const int i = __builtin_ctzll(left) + 1, n = length(i);
+    const int64_t s = slots[i];
+    const int off = (int)(s & (page - 1));
+    if (((off + n + 3) / 4 - off / 4) * (p.c.dim / 8) <= 64)
+      append_run<T, false>(p, h, is_v, t0 + i - 1, s, n, wave_max, vt);
+    else if (lane == 0)
+      atomicOr((unsigned long long*)&long_runs, left & -left);
+  }
+  __syncthreads();
+  for (uint64_t left = long_runs; left != 0u; left &= left - 1) {
+    const int i = __builtin_ctzll(left) + 1, n = length(i);
+    append_run<T, true>(p, h, is_v, t0 + i - 1, slots[i], n, wave_max, vt);
     __syncthreads();  // wave_max and vt are read before the next run
   }
 }
@@ -310,19 +338,24 @@ __global__ __launch_bounds__(kMaxThreads) void kv_append(KvAppendParams p, int w
 }  // namespace
 
 hipError_t launch_kv_append(const KvAppendParams& p, hipStream_t stream) {
-  // A step of single tokens has a run in each: a workgroup for each token.  Long runs: one for the runs of 64 tokens.
-  const int window = p.tokens <= 1024 ? 1 : 64;
+  // A workgroup for 64 tokens, or fewer where that leaves less than 2,048 workgroups: runs of single tokens have a wave
+  // each, and one behind the other takes 3 us (64 tokens x 8 heads in 64 pages: 6.6 us with a workgroup for each, 54 for
+  // all 64 in one; 1,024 tokens x 8 heads: in runs of 64 13.5 for 8 a workgroup, 40 for one; in single ones 23 and 44).
+  const int64_t halves = 2 * p.tokens * p.c.heads / 2048;
+  int window = 1;
+  while (window < 64 && 2 * window <= halves) window *= 2;
   const int64_t wgs = (p.tokens + window - 1) / window;
   if (wgs > 0x7fffffff || p.c.heads > 65535) return hipErrorInvalidValue;
   const dim3 grid((unsigned)wgs, (unsigned)p.c.heads, 2);
   const int items = (p.c.dim << p.c.page_log2) / 32;
-  const dim3 block(window == 1 || items < 64 ? 64 : items);
+  const dim3 block(items < 64 ? 64 : items);
+  const size_t lds = p.c.dim * ((1 << p.c.page_log2) / 4 + 1) * sizeof(uint32_t);
   if (p.dtype == 0)
-    hipLaunchKernelGGL(kv_append<__bf16>, grid, block, 0, stream, p, window);
+    hipLaunchKernelGGL(kv_append<__bf16>, grid, block, lds, stream, p, window);
   else if (p.dtype == 1)
-    hipLaunchKernelGGL(kv_append<_Float16>, grid, block, 0, stream, p, window);
+    hipLaunchKernelGGL(kv_append<_Float16>, grid, block, lds, stream, p, window);
   else
-    hipLaunchKernelGGL(kv_append<float>, grid, block, 0, stream, p, window);
+    hipLaunchKernelGGL(kv_append<float>, grid, block, lds, stream, p, window);
   return hipGetLastError();
 }
 

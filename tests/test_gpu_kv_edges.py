@@ -1,10 +1,13 @@
 """Calls at the edges of what the cache's attention and the rotary embedding are documented to take: rows in front of
 the first request, captured backward passes beside living graphs, pieces that do not line up."""
+import random
+
 import pytest
 import torch
 
 from pasa_amd.kv_cache import cached_attention
 from pasa_amd.rotary import RotaryAxes, rope_axes
+from test_gpu_kv_append import check as append_check, make_cache, tokens
 from test_gpu_kv_attention import check, make
 from test_gpu_rotary import close as against, make as values
 
@@ -86,3 +89,28 @@ def test_whole_pieces_and_others(device, dtype, pairing, T, H, D, dims):
     close(rope_axes(off, None, pos, axes)[0], x, pos, axes, inverse=False, what="an element off")
     rope_axes(off, None, pos, axes, inplace=True)
     close(off, x, pos, axes, inverse=False, what="an element off, in place")
+
+
+@pytest.mark.parametrize("T,H,D,page,lengths", [(2500, 8, 128, 64, [1, 1, 2, 5, 13, 16, 40, 64]), (2500, 8, 64, 16, [1, 3, 15, 16]),
+                                                (5000, 16, 128, 16, [1, 1, 1, 2]), (5000, 16, 64, 128, [1, 60, 128]), (1100, 2, 96, 32, [1, 7])])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_runs_in_one_append(device, dtype, T, H, D, page, lengths):
+    """Workgroups that take several tokens: short runs side by side, long ones together, a page to each."""
+    rng = random.Random(T + page)
+    slots = []
+    while len(slots) < T:
+        n = min(rng.choice(lengths), T - len(slots), page)
+        slots.append((n, rng.randrange(page - n + 1)))
+        slots += [None] * (n - 1)
+    runs = [s for s in slots if s is not None]
+    ids = rng.sample(range(len(runs) + 2), len(runs))
+    slots = [i * page + at + j for i, (n, at) in zip(ids, runs) for j in range(n)]
+    for i in rng.sample(range(T), 5):
+        slots[i] = rng.choice([-1, 10 ** 13])  # ends a run: what is left of it is skipped too
+        rest = i + 1
+        while rest < T and slots[rest] % page != 0 and slots[rest] // page == (slots[i - 1] // page if i else -1):
+            slots[rest] = -1
+            rest += 1
+    c = make_cache(device, len(runs) + 2, H, D, page, seed=T)
+    k, v = tokens(T, H, D, dtype, T, spread=2.0)
+    append_check(c, k, v, slots, f"{len(runs)} runs of {T} tokens, page {page}")
