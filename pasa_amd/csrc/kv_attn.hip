@@ -71,7 +71,6 @@ __device__ __forceinline__ uint32_t finite_bytes(uint32_t w) {
 // The requests' first rows of q, clamped to the rows that there are.
 // (tokens * q_heads < 2^31: row numbers fit 32 bits.)
 __device__ __forceinline__ int first_token(const KvAttnParams& p, int r) {
-  if (p.cu_q == nullptr) return r * p.per_request;
   return min(max(p.cu_q[r], 0), (int)p.tokens);
 }
 
@@ -86,6 +85,17 @@ template <int TILE>
 __device__ __forceinline__ TileOf find_tile(const KvAttnParams& p, int id) {
   // The last request whose number is at or before id: 64 candidates at a time, one for each lane, which in the last round
   // (the only one for up to 63 requests) also has its request's length.
+  TileOf t;
+  if (p.cu_q == nullptr) {  // the same for all: no more numbers than tiles
+    t.rows = p.per_request * p.group;
+    const int each = (t.rows + TILE - 1) / TILE;
+    t.r = id / each;
+    t.tok0 = t.r * p.per_request;
+    t.row0 = (id - t.r * each) * TILE;
+    t.raw_len = max(p.lens[t.r], 0);
+    t.front = 0;
+    return t;
+  }
   const int lane = threadIdx.x & 63;
   int lo = 0, n = p.requests + 1;
   auto number = [&](int first, int r) { return first * p.group / TILE + r; };
@@ -98,7 +108,6 @@ __device__ __forceinline__ TileOf find_tile(const KvAttnParams& p, int id) {
   const int at = min(lo + lane, p.requests);
   const int first = first_token(p, at), len = p.lens[min(at, p.requests - 1)];
   const int i = max(__popcll(__ballot(lane < n && number(first, at) <= id)), 1) - 1;
-  TileOf t;
   t.r = lo + i;
   t.tok0 = __builtin_amdgcn_readlane(first, i);
   const int tok1 = t.r == p.requests ? (int)p.tokens : i < 63 ? __builtin_amdgcn_readlane(first, min(i + 1, 63)) : first_token(p, t.r + 1);
@@ -287,7 +296,9 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
 // ---- few rows --------------------------------------------------------------------
 // A workgroup has 16 * NQ rows of one key head; its eight waves take the 64-key tiles in turn, straight from memory into
 // registers, and their sums are joined in LDS.  blockIdx.z: a part of the keys.  Bound by the bytes of the keys: eight
-// waves a compute unit, each with a tile of 16 KB in flight, ask for more than HBM gives.
+// waves a compute unit, each with a tile of 16 KB in flight, ask for more than HBM gives.  2 tokens x 75,600 keys of 40
+// heads of 128 channels: 270 us with the join, 5.7 TB/s where a plain read of as much reaches 6.2; 64 tokens to ragged
+// lengths up to 8,192, 8 heads: 131 us, 4.3 TB/s (one round of workgroups of unequal lengths).
 template <typename E, int DIM, int NQ>
 __global__ __launch_bounds__(512, 2) void kv_attn_rows(KvAttnParams p) {
   constexpr int WAVES = 8;
@@ -541,9 +552,9 @@ __global__ __launch_bounds__(512, 2) void kv_attn_rows(KvAttnParams p) {
 // Bound by the SIMDs' issue: an MFMA of 16 cycles has 32 rows x 64 keys x 32 channels / 4, and between two of them go the
 // scale, exponential, sum, maximum and rounding of two scores (about 11 cycles at head dim 128, twice that at 64) and the
 // LDS reads.  3,600 tokens x 75,600 keys of 40 heads of 128 channels: 14.3 ms with 16-row tiles, 9.65 with 128 rows, 6.2
-// with 256 (half the LDS reads and widening a row) and the scores a tile ahead, 5.3 with K three tiles deep: 1.05 PFLOP/s,
-// where the chip's matrix products reach 1.37.  12 requests of 1,500 tokens, 32 heads of 64 channels, a causal window of
-// 4,096 on 6,000 keys: 0.26 ms, 0.62 PFLOP/s.
+// with 256 (half the LDS reads and widening a row) and the scores a tile ahead, 5.2 with K three tiles deep: 1.08 PFLOP/s,
+// where the chip's matrix products reach 1.37.  12 requests of 1,500 tokens on 6,000 keys, 32 heads of 64 channels: 1.13 ms,
+// 0.78 PFLOP/s.
 template <int DIM, int WAVES>
 struct KvTile {
   static constexpr int ROWS = 32 * WAVES;
@@ -1064,10 +1075,13 @@ __global__ __launch_bounds__(256) void kv_attn_join(KvAttnParams p) {
   if (lane == 0 && p.lse) p.lse[row] = row_lse(top, l);
 }
 
-// Tile numbers that a head of the launch has.  Some have no rows, often every second one (a request of less than a tile):
+// Tile numbers that a head of the launch has.  With row starts some have no rows, often every second one (a request of less than a tile):
 // their number is odd, so that those that have some fall to all XCDs and compute units, which take workgroups in turn
 // (1 request, 96 rows a head, 32,768 keys of 40 heads: 206 us at 2 numbers a head, 129 at 3).
-int64_t tile_numbers(const KvAttnParams& p, int rows) { return (p.tokens * p.group / rows + p.requests + 1) | 1; }
+int64_t tile_numbers(const KvAttnParams& p, int rows) {
+  if (p.cu_q == nullptr) return (int64_t)p.requests * (((int64_t)p.per_request * p.group + rows - 1) / rows);
+  return (p.tokens * p.group / rows + p.requests + 1) | 1;
+}
 
 template <typename E, int DIM, int NQ>
 hipError_t launch_rows(const KvAttnParams& p, hipStream_t stream) {
@@ -1108,25 +1122,28 @@ hipError_t launch_any(const KvAttnParams& p, int rows, hipStream_t stream) {
 
 }  // namespace
 
-// Tile and parts of the keys, from the sizes that the host knows.  Tiles of 16 and 32 rows are bound by the bytes of the
-// keys, of 128 and 256 by the matrix units (rates of long runs, in us).  The workgroups run in rounds of as many as the
+// Tile and parts of the keys, from the sizes that the host knows.  Tiles of 16 rows are bound by the bytes of the keys, of
+// 32 by those and the widening, of 128 and 256 by the matrix units (rates of long runs, in us).  The tile is the one that
+// holds a request's rows, with the best parts of each measured: 16 requests, 4,096 keys of 8 heads of 128 channels, 12 rows
+// a request and key head: 30 us with 16, 33 with 32 rows; 24: 45, 34; 48: 32 rows 48, 128 rows 54; 96: 80, 59; 128: 128
+// rows 62, 256 rows 81; 160: 95, 84; 512: 148, 130 us.  The workgroups run in rounds of as many as the
 // chip holds at once; more parts of the keys make the last round shorter, but a workgroup begins and ends for some us and
 // its sums pass through memory and a second launch.  Parts are added while that gains 3%: workgroups that sweep the same
 // keys at the same time share them in L2, and the more rounds there are the further they drift apart (3,600 tokens x
-// 75,600 of 40 heads: 6.46 ms whole, 5.30 in 2 parts, 5.44 in 4, 5.80 in 5).
+// 75,600 of 40 heads: 6.08 ms whole, 5.00 in 2 parts, 5.07 in 4, 5.36 in 5).
 KvAttnPlan kv_attn_plan(int64_t tokens, int requests, int q_heads, int kv_heads, int dim, int64_t max_kv) {
   const int group = q_heads / kv_heads;
   const int64_t mean = (tokens * group + requests - 1) / requests;
   KvAttnPlan plan;
-  plan.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 128 || dim != 128 ? 128 : 256;
+  plan.rows = mean <= 16 ? 16 : mean <= 64 ? 32 : mean <= 128 || dim != 128 ? 128 : 256;
   plan.splits = 1;
   const bool few = plan.rows <= 32;
   // Four tiles a wave at most: one launch (1 token to 1,560 of 12 heads: 15.6 us on the GPU, 10 in four parts and their
   // join, but 19.7 us a call against 23, which is what the two launches cost the host).
   if (few && max_kv <= 2048) return plan;
-  const double wgs = (double)((mean + plan.rows - 1) / plan.rows) * requests * kv_heads;
+  const double tiles = (double)((mean + plan.rows - 1) / plan.rows), wgs = tiles * requests * kv_heads;
   const double slots = plan.rows == 128 ? 512 : 256;
-  const double work_us = few ? 2.0 * requests * max_kv * kv_heads * dim / (plan.rows == 16 ? 5.5e6 : 3.6e6) : 4.0 * tokens * max_kv * q_heads * dim / 1.1e9;
+  const double work_us = few ? 2.0 * tiles * requests * max_kv * kv_heads * dim / (plan.rows == 16 ? 5.5e6 : 3.6e6) : 4.0 * tokens * max_kv * q_heads * dim / 1.1e9;
   const double part_us = 2.0 * tokens * q_heads * (dim + 2) * sizeof(float) / 4.5e6;  // written and read
   const int64_t most = (max_kv + 511) / 512 < 64 ? (max_kv + 511) / 512 : 64;        // eight tiles a part at least
   double best = 0.0;

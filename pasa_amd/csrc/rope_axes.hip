@@ -7,7 +7,8 @@
 // either way, and only then rounded to fp32, so a position far out costs no accuracy; the rotation is fp32 and
 // rounded once.
 //
-// Bound by HBM: each channel is read once and written once, positions are 12 bytes a token.  The angles' sines are
+// Bound by HBM: each channel is read once and written once, positions are 12 bytes a token (75,600 tokens, 2 x 40 heads
+// of 128 channels in bf16: 578 us, 5.4 TB/s; a plain copy of as much reaches 4.9).  The angles' sines are
 // computed where they are used, once for all heads that a wave (or, element by element, a workgroup) takes.
 #include <math.h>
 
@@ -70,7 +71,8 @@ __global__ __launch_bounds__(256) void rope_axes_scalar(RopeAxesParams p) {
   }
 }
 
-// 16 bytes at a time.  A wave takes a token, or a part of its heads: a lane has one 16-byte unit of a head's channels
+// 16 bytes at a time, where the channels, strides and pairs allow it (64 tokens of 48 heads: 4.5 us, element by element
+// 8.2; 8,192 tokens: 33 and 72).  A wave takes a token, or a part of its heads: a lane has one 16-byte unit of a head's channels
 // (HALVES: two, whose channels are each other's pairs), 64 / units heads lie side by side in the wave.  The lanes share
 // out the pairs' angles, and through LDS each gets the sines of its own, which stay in registers for all heads.
 template <typename T, bool HALVES>
@@ -160,7 +162,8 @@ void launch(const RopeAxesParams& p, hipStream_t stream) {
   }
   const int v = 16 / (int)sizeof(T);
   const int units = (p.halves ? p.D - p.pairs : p.D) / v, rows = 64 / units;
-  // Few tokens: their heads are shared out until the chip has its waves, each computing the sines again.
+  // Few tokens: their heads are shared out until the chip has its waves, each computing the sines again (64 tokens of 48
+  // heads: 6.8 us with a wave to a token, 4.5 with 16; 8,192 tokens: 33 and 66).
   const int most = max(p.t[0].heads, p.t[1].heads);
   int parts = 1;
   while (parts < 16 && all * parts < 8192 && parts * rows < most) parts *= 2;
