@@ -7,5 +7,7 @@ Kernels live in libpasa_amd.so (C ABI, include/pasa.h), built in-tree by
 * ``pasa_amd.placement``  frame-major <-> token-major permutation
 * ``pasa_amd.processors`` Wan / HunyuanVideo attention processors and installers
 * ``pasa_amd.density``    per-timestep density tables
+* ``pasa_amd.rotary``     rotary embedding from positions on several axes, with its gradient
+* ``pasa_amd.kv_cache``   a paged key/value cache in 8 bits: block tables, append, attention
 """
 __version__ = "0.1.0"

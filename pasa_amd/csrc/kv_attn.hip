@@ -1138,8 +1138,8 @@ KvAttnPlan kv_attn_plan(int64_t tokens, int requests, int q_heads, int kv_heads,
   plan.rows = mean <= 16 ? 16 : mean <= 64 ? 32 : mean <= 128 || dim != 128 ? 128 : 256;
   plan.splits = 1;
   const bool few = plan.rows <= 32;
-  // Four tiles a wave at most: one launch (1 token to 1,560 of 12 heads: 15.6 us on the GPU, 10 in four parts and their
-  // join, but 19.7 us a call against 23, which is what the two launches cost the host).
+  // Four tiles a wave at most: one launch (1 token to 1,560 of 12 heads: 14.0 us on the GPU, 10.5 in four parts with their
+  // join, but a second launch costs the host about 4 us of a call that takes it 13).
   if (few && max_kv <= 2048) return plan;
   const double tiles = (double)((mean + plan.rows - 1) / plan.rows), wgs = tiles * requests * kv_heads;
   const double slots = plan.rows == 128 ? 512 : 256;
