@@ -1,14 +1,16 @@
 """Calls at the edges of what the cache's attention and the rotary embedding are documented to take: rows in front of
-the first request, captured backward passes beside living graphs, pieces that do not line up."""
+the first request, requests of one length, appends of many runs, captured backward passes beside living graphs, pieces
+that do not line up."""
 import random
 
 import pytest
 import torch
 
+from oracle import kv_oracle as K
 from pasa_amd.kv_cache import cached_attention
 from pasa_amd.rotary import RotaryAxes, rope_axes
 from test_gpu_kv_append import check as append_check, make_cache, tokens
-from test_gpu_kv_attention import check, make
+from test_gpu_kv_attention import check, compare, make
 from test_gpu_rotary import close as against, make as values
 
 pytestmark = pytest.mark.gpu
@@ -114,3 +116,18 @@ def test_many_runs_in_one_append(device, dtype, T, H, D, page, lengths):
     c = make_cache(device, len(runs) + 2, H, D, page, seed=T)
     k, v = tokens(T, H, D, dtype, T, spread=2.0)
     append_check(c, k, v, slots, f"{len(runs)} runs of {T} tokens, page {page}")
+
+
+# (heads of q, of k, head dim, new, cached): a part of a tile, several, a part of the last; of 16, 32, 128, 256 rows; split.
+@pytest.mark.parametrize("Hq,Hk,D,new,kv", [
+    (2, 2, 128, 3, 70), (8, 2, 64, 5, 700), (8, 1, 128, 7, 5000), (8, 1, 64, 20, 300), (8, 1, 128, 20, 900),
+    (8, 1, 128, 70, 6000), (4, 1, 64, 100, 5000), (1, 1, 128, 300, 310)])
+@pytest.mark.parametrize("window", [None, 100])
+def test_requests_of_one_length(device, Hq, Hk, D, new, kv, window):
+    """Without row starts: every request has its own tiles, and the result is that with row starts, within the bounds."""
+    c, q, tables, kv, cu = make(device, [kv, kv - 7, kv - new], [new] * 3, Hq, Hk, D, 32, torch.float16, seed=new)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
+    o, lse = cached_attention(q, c, i32(tables), i32(kv), causal=True, window=window, return_lse=True)
+    torch.cuda.synchronize()
+    want = K.attention(q.cpu(), c.k.cpu(), c.v.cpu(), c.k_exp.cpu(), c.v_exp.cpu(), tables, kv, cu, D ** -0.5, True, window)
+    compare(o, lse, *want, f"{new} tokens each")
